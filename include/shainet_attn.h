@@ -372,6 +372,88 @@ int shainet_attn_decode_noalloc(const float* q_dev, const float* k_cache_dev, co
                                 float* out_dev, int start_pos, int num_heads, int heads_per_kv, int head_dim,
                                 int capacity, float scale, void* stream);
 
+/* ---- paged batches: keys and values of many requests in pages of one pool, for servers whose requests come and go
+ * (no counterpart in the reference, which holds one growing cache per block, llama_block.cr:45-56).  All of it works on
+ * the caller's device memory: a pool per block, k_pages and v_pages [num_pages, num_kv_heads, page_rows, head_dim] in
+ * the element format of SHAINET_ATTN_KV_*; and, shared by all blocks, block_table [requests, table_width] int32 whose
+ * row r lists the pages of request r in order, and lens [requests] int32.  Position p of request r lies in row
+ * p % page_rows of page block_table[r][p / page_rows]; the slot of a position is page * page_rows + row.  A page belongs
+ * to one request where rows are written into it; pages that are only read may be shared.  num_pages * page_rows is at
+ * most 2^31 - 1, page_rows 1 .. 4096.
+ *
+ * plan_dev: one step of the page tables, on the device and in one launch.  Request r holds lens[r] positions; delta[r]
+ * positions are added (> 0) or the newest ones dropped (< 0; -lens[r] ends the request).  The free pages are a stack,
+ * free_pages[0 .. free_count): pages that requests no longer need are pushed in the order of the requests, a request's
+ * by their place in its table; then requests that grow pop theirs in the order of the requests, by place in the table.
+ * Written: the new table cells, the stack, lens_out = lens + delta, free_count_out, first [requests + 1] (the exclusive
+ * sums of max(delta, 0): where a request's new tokens start), slots [max_tokens] (the slot of every new token, -1 behind
+ * the last one) and status [2].  Table cells and stack entries that are not in use keep what they held.  lens_out may be
+ * lens and free_count_out may be free_count (a captured step advances its own state); no other two arrays may overlap.
+ * Nothing is changed (lens_out = lens, free_count_out = free_count, first 0, slots -1) and status[0] is not 0 where
+ * the step cannot be taken: SHORT, status[1] pages are missing; LENGTH, request status[1] has a length below 0 or above
+ * table_width * page_rows before or after the step; TOKENS, the status[1] new tokens are more than max_tokens; STACK,
+ * free_count[0] = status[1] is outside [0, num_pages], or the stack would outgrow free_pages [num_pages].
+ * requests is at most SHAINET_ATTN_PAGED_MAX_REQUESTS.  free_pages holds each free page once. */
+#define SHAINET_ATTN_PAGED_MAX_REQUESTS 8192
+#define SHAINET_ATTN_PLAN_OK 0
+#define SHAINET_ATTN_PLAN_SHORT 1
+#define SHAINET_ATTN_PLAN_LENGTH 2
+#define SHAINET_ATTN_PLAN_TOKENS 3
+#define SHAINET_ATTN_PLAN_STACK 4
+int shainet_attn_paged_plan_dev(shainet_attn_ctx* ctx, int requests, const int32_t* lens, const int32_t* delta,
+                                int32_t* block_table, int table_width, int page_rows, int32_t* free_pages, int num_pages,
+                                const int32_t* free_count, int32_t* lens_out, int32_t* free_count_out, int32_t* first,
+                                int32_t* slots, int max_tokens, int32_t* status, void* stream);
+/* The head layout and the workspace of the calls below.  Calls that use one handle run one behind another: on one
+ * stream, or ordered by events or graph edges.  Streams or graphs that may run at the same time take a handle each.
+ * head_dim is 64 or 128, any number of query heads per kv head. */
+typedef struct shainet_attn_paged shainet_attn_paged;
+int shainet_attn_paged_create(shainet_attn_ctx* ctx, shainet_attn_paged** out, int num_heads, int num_kv_heads,
+                              int head_dim, int page_rows, int format);
+int shainet_attn_paged_destroy(shainet_attn_paged* paged);
+/* One decode token for each request, the paged form of shainet_attn_forward_batched_dev: q [requests, q_dim], k_new /
+ * v_new [requests, kv_dim] are raw projection outputs, out [requests, q_dim].  lens counts the new token: its position
+ * is lens[r] - 1, its rotated k row and its v row are written there, and it sees the positions 0 .. lens[r] - 1.  kv is
+ * the block's cache: RoPE table, norm weights, biases and head layout are its own, its rows are not touched.
+ * lens[r] == 0 is a padded row: nothing is written into pages, its out row is zeros.  Lengths are read on the device, so
+ * the call can be captured and replayed as requests grow.  A length that the table cannot hold makes a row of zeros, a
+ * table cell outside the pool is not followed (that request's out row is then unspecified); either is reported as
+ * SHAINET_ATTN_E_INVALID by the next blocking call on ctx after the stream was synchronised.  Rows of pages behind a
+ * request's last position are never used, whatever they hold.  Arithmetic is fp32 or better over the rows as the pages
+ * hold them; results do not depend on what else is in the batch than through the split of a request's positions. */
+int shainet_attn_paged_decode_dev(shainet_attn_ctx* ctx, shainet_attn_paged* paged, const shainet_attn_kv* kv,
+                                  void* k_pages, void* v_pages, int num_pages, const float* q_dev, const float* k_new_dev,
+                                  const float* v_new_dev, float* out_dev, const int32_t* block_table, int table_width,
+                                  const int32_t* lens, int requests, float scale, void* stream);
+/* Between pages and a contiguous cache of the same layout and format, on which prompts and short turns run
+ * (shainet_attn_forward_dev).  scatter: rows row0 .. row0 + rows - 1 of kv go to slots[0 .. rows) (distinct; a negative
+ * slot is skipped).  gather: positions 0 .. rows - 1 of the request whose table row is table_row become the rows of kv,
+ * whose length becomes rows; kv grows if it has to, which a stream that is being captured does not allow.  A slot or
+ * page outside the pool is skipped and reported as above. */
+int shainet_attn_paged_scatter_dev(shainet_attn_ctx* ctx, shainet_attn_paged* paged, const shainet_attn_kv* kv, void* k_pages,
+                                   void* v_pages, int num_pages, const int32_t* slots, int row0, int rows, void* stream);
+int shainet_attn_paged_gather_dev(shainet_attn_ctx* ctx, shainet_attn_paged* paged, shainet_attn_kv* kv, const void* k_pages,
+                                  const void* v_pages, int num_pages, const int32_t* table_row, int rows, void* stream);
+
+/* ---- 4-bit weights with group scales, beside the Q8_0 weights (no counterpart in the reference): weight [K, N] as
+ * nibbles 0 .. 15 that stand for -8 .. 7 and one fp32 scale per `group` (32, 64 or 128) consecutive K of an output; the
+ * last group of an output may be short.  Exchange layout: packed [N, ceil(K/2)], K = 2j in the low and 2j + 1 in the
+ * high nibble of byte j (the high nibble behind an odd K is ignored and exported as 8), scales [N, ceil(K/group)].
+ * q4_create quantises an fp32 matrix [K, N] as the Q8_0 one does: scale = max|w| / 7 (1 for an all-zero group), value =
+ * round(w * (1 / scale)), ties to even.  create_raw takes host arrays, create_dev device arrays (read on the context's
+ * stream before it returns).  All of them lay the nibbles out anew for the kernel.
+ * y[rows, N] = x[rows, K] . dequant(W), fp32 sums of exact products; x is not rounded. */
+typedef struct shainet_attn_q4 shainet_attn_q4;
+int shainet_attn_q4_create(shainet_attn_ctx* ctx, shainet_attn_q4** out, const float* w_host, int K, int N, int group);
+int shainet_attn_q4_create_raw(shainet_attn_ctx* ctx, shainet_attn_q4** out, const uint8_t* packed_host,
+                               const float* scales_host, int K, int N, int group);
+int shainet_attn_q4_create_dev(shainet_attn_ctx* ctx, shainet_attn_q4** out, const uint8_t* packed_dev,
+                               const float* scales_dev, int K, int N, int group);
+int shainet_attn_q4_destroy(shainet_attn_q4* w);
+int shainet_attn_q4_export(shainet_attn_q4* w, uint8_t* packed_host, float* scales_host);
+int shainet_attn_q4_gemv_dev(shainet_attn_ctx* ctx, const shainet_attn_q4* w, const float* x_dev, float* y_dev, int rows,
+                             void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -11,6 +11,7 @@ LIB_PATH = os.path.join(PKG, "lib", "libshainet_attn.so")
 
 OK = 0
 E_INVALID, E_CUDA, E_NOMEM, E_UNSUPPORTED, E_DEVICE_WAIT, E_STATE = -1, -2, -3, -4, -5, -6
+PLAN_OK, PLAN_SHORT, PLAN_LENGTH, PLAN_TOKENS, PLAN_STACK = 0, 1, 2, 3, 4   # status[0] of a page plan
 F_GENERIC, F_SPLITK, F_TENSOR, F_UNFUSED, F_INPUTS_READY, F_TICKET_MERGE, F_TENSOR_1CTA = 1, 2, 4, 8, 16, 32, 64
 
 _F = C.POINTER(C.c_float)
@@ -81,6 +82,18 @@ SIGNATURES = {
     "shainet_attn_decoder_run": (C.c_int, [_P, _P, C.POINTER(C.c_int32), C.c_int, _F, C.POINTER(C.c_int32)]),
     "shainet_attn_decoder_generate": (C.c_int, [_P, _P, C.POINTER(C.c_int32), C.c_int, C.c_int, C.POINTER(C.c_int32)]),
     "shainet_attn_decode_noalloc": (C.c_int, [_P, _P, _P, _P, C.c_int, C.c_int, C.c_int, C.c_int, C.c_int, C.c_float, _P]),
+    "shainet_attn_paged_plan_dev": (C.c_int, [_P, C.c_int, _P, _P, _P, C.c_int, C.c_int, _P, C.c_int, _P, _P, _P, _P, _P, C.c_int, _P, _P]),
+    "shainet_attn_paged_create": (C.c_int, [_P, C.POINTER(_P), C.c_int, C.c_int, C.c_int, C.c_int, C.c_int]),
+    "shainet_attn_paged_destroy": (C.c_int, [_P]),
+    "shainet_attn_paged_decode_dev": (C.c_int, [_P, _P, _P, _P, _P, C.c_int, _P, _P, _P, _P, _P, C.c_int, _P, C.c_int, C.c_float, _P]),
+    "shainet_attn_paged_scatter_dev": (C.c_int, [_P, _P, _P, _P, _P, C.c_int, _P, C.c_int, C.c_int, _P]),
+    "shainet_attn_paged_gather_dev": (C.c_int, [_P, _P, _P, _P, _P, C.c_int, _P, C.c_int, _P]),
+    "shainet_attn_q4_create": (C.c_int, [_P, C.POINTER(_P), _F, C.c_int, C.c_int, C.c_int]),
+    "shainet_attn_q4_create_raw": (C.c_int, [_P, C.POINTER(_P), _P, _F, C.c_int, C.c_int, C.c_int]),
+    "shainet_attn_q4_create_dev": (C.c_int, [_P, C.POINTER(_P), _P, _P, C.c_int, C.c_int, C.c_int]),
+    "shainet_attn_q4_destroy": (C.c_int, [_P]),
+    "shainet_attn_q4_export": (C.c_int, [_P, _P, _F]),
+    "shainet_attn_q4_gemv_dev": (C.c_int, [_P, _P, _P, _P, C.c_int, _P]),
     "kv_cache_append_f32": (None, [_P, _P, _P, C.c_int, C.c_int, C.c_int, C.c_int, C.c_int]),
     "attention_kv_f32": (None, [_P, _P, _P, _P, _P, C.c_int, C.c_int, C.c_int, C.c_int, C.c_int, C.c_int,
                                 C.c_float]),

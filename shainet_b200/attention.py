@@ -308,6 +308,63 @@ def forward_batched_dev(ctx: AttnContext, caches, q_ptr: int, k_ptr: int, v_ptr:
                                                  _stream_arg(stream)))
 
 
+def plan_pages_dev(ctx: AttnContext, requests: int, lens_ptr: int, delta_ptr: int, block_table_ptr: int, table_width: int,
+                   page_rows: int, free_pages_ptr: int, num_pages: int, free_count_ptr: int, lens_out_ptr: int,
+                   free_count_out_ptr: int, first_ptr: int, slots_ptr: int, max_tokens: int, status_ptr: int, stream=None):
+    """One step of the page tables of a batch on the device: pages pushed and popped, lengths, offsets and slots of the
+    new tokens.  int32 device pointers; ``status`` receives ``_lib.PLAN_*`` and its detail."""
+    check(ctx.L.shainet_attn_paged_plan_dev(ctx.h, requests, lens_ptr, delta_ptr, block_table_ptr, table_width, page_rows,
+                                            free_pages_ptr, num_pages, free_count_ptr, lens_out_ptr, free_count_out_ptr,
+                                            first_ptr, slots_ptr, max_tokens, status_ptr, _stream_arg(stream)))
+
+
+def _cache_of(attn):
+    return attn.cache if isinstance(attn, LlamaAttention) else attn
+
+
+class PagedAttention:
+    """Attention and copies over keys and values that lie in pages of the caller's pool, [num_pages, num_kv_heads,
+    page_rows, head_dim] per tensor.  One object serves calls that run one behind another; streams or graphs that may
+    run at the same time take one each.  ``attn`` is the block's ``LlamaAttention`` (or its ``KVCache``): decode takes
+    RoPE, norms and biases from it, the copies its rows."""
+
+    def __init__(self, ctx: AttnContext, num_heads: int, num_kv_heads: int, head_dim: int, page_rows: int = 16,
+                 kv_format: str = "f32"):
+        if kv_format not in KV_FORMATS:
+            raise ValueError(f"kv_format must be one of {sorted(KV_FORMATS)}")
+        self.ctx, self.L = ctx, ctx.L
+        self.num_heads, self.num_kv_heads, self.head_dim, self.page_rows = num_heads, num_kv_heads, head_dim, page_rows
+        h = C.c_void_p()
+        check(self.L.shainet_attn_paged_create(ctx.h, C.byref(h), num_heads, num_kv_heads, head_dim, page_rows,
+                                               KV_FORMATS[kv_format]))
+        self.h = h
+
+    def decode_dev(self, attn, k_pages_ptr: int, v_pages_ptr: int, num_pages: int, q_ptr: int, k_ptr: int, v_ptr: int,
+                   out_ptr: int, block_table_ptr: int, table_width: int, lens_ptr: int, requests: int, scale: float,
+                   stream=None):
+        """One decode token for each request; ``lens`` counts it, 0 is a padded row."""
+        check(self.L.shainet_attn_paged_decode_dev(self.ctx.h, self.h, _cache_of(attn).h, k_pages_ptr, v_pages_ptr, num_pages,
+                                                   q_ptr, k_ptr, v_ptr, out_ptr, block_table_ptr, table_width, lens_ptr,
+                                                   requests, scale, _stream_arg(stream)))
+
+    def scatter_dev(self, attn, k_pages_ptr: int, v_pages_ptr: int, num_pages: int, slots_ptr: int, row0: int, rows: int,
+                    stream=None):
+        """Rows [row0, row0 + rows) of the block's cache into the slots (negative: skipped)."""
+        check(self.L.shainet_attn_paged_scatter_dev(self.ctx.h, self.h, _cache_of(attn).h, k_pages_ptr, v_pages_ptr, num_pages,
+                                                    slots_ptr, row0, rows, _stream_arg(stream)))
+
+    def gather_dev(self, attn, k_pages_ptr: int, v_pages_ptr: int, num_pages: int, table_row_ptr: int, rows: int,
+                   stream=None):
+        """Positions [0, rows) of the request with this table row become the rows of the block's cache."""
+        check(self.L.shainet_attn_paged_gather_dev(self.ctx.h, self.h, _cache_of(attn).h, k_pages_ptr, v_pages_ptr, num_pages,
+                                                   table_row_ptr, rows, _stream_arg(stream)))
+
+    def close(self):
+        if getattr(self, "h", None):
+            check(self.L.shainet_attn_paged_destroy(self.h))
+            self.h = None
+
+
 class Q8Weight:
     """The reference's ``QuantizedCudaMatrix`` (src/shainet/math/quantized_cuda_matrix.cr): a
     weight [K, N] held on the device as Q8_0.  ``from_simple`` quantises an fp32 matrix,
@@ -352,6 +409,54 @@ class Q8Weight:
     def close(self):
         if getattr(self, "h", None):
             check(self.ctx.L.shainet_attn_q8_destroy(self.h))
+            self.h = None
+
+
+class Q4Weight:
+    """A weight [K, N] held on the device as 4-bit values with one fp32 scale per ``group`` inputs of an output (no
+    counterpart in the reference).  ``from_simple`` quantises an fp32 matrix, ``from_quantized`` takes host arrays,
+    nibbles [N, ceil(K/2)] and scales [N, ceil(K/group)], ``from_device`` the same as device pointers."""
+
+    def __init__(self, ctx: AttnContext, handle, K: int, N: int, group: int):
+        self.ctx, self.h, self.K, self.N, self.group = ctx, handle, K, N, group
+
+    @classmethod
+    def from_simple(cls, ctx: AttnContext, w, group: int = 32):
+        w = _f32(w)
+        h = C.c_void_p()
+        check(ctx.L.shainet_attn_q4_create(ctx.h, C.byref(h), _fp(w), w.shape[0], w.shape[1], group))
+        return cls(ctx, h, w.shape[0], w.shape[1], group)
+
+    @classmethod
+    def from_quantized(cls, ctx: AttnContext, packed, scales, K: int, group: int = 32):
+        packed, scales = np.ascontiguousarray(packed, np.uint8), _f32(scales)
+        N = packed.shape[0]
+        if packed.shape != (N, (K + 1) // 2) or group <= 0 or scales.shape != (N, (K + group - 1) // group):
+            raise ValueError("packed must be [N, ceil(K/2)]; scales [N, ceil(K/group)]")
+        h = C.c_void_p()
+        check(ctx.L.shainet_attn_q4_create_raw(ctx.h, C.byref(h), packed.ctypes.data_as(C.c_void_p), _fp(scales), K, N, group))
+        return cls(ctx, h, K, N, group)
+
+    @classmethod
+    def from_device(cls, ctx: AttnContext, packed_ptr: int, scales_ptr: int, K: int, N: int, group: int = 32):
+        """Device arrays; they are read before this returns and not kept."""
+        h = C.c_void_p()
+        check(ctx.L.shainet_attn_q4_create_dev(ctx.h, C.byref(h), packed_ptr, scales_ptr, K, N, group))
+        return cls(ctx, h, K, N, group)
+
+    def export(self):
+        packed = np.empty((self.N, (self.K + 1) // 2), np.uint8)
+        s = np.empty((self.N, (self.K + self.group - 1) // self.group), np.float32)
+        check(self.ctx.L.shainet_attn_q4_export(self.h, packed.ctypes.data_as(C.c_void_p), _fp(s)))
+        return packed, s
+
+    def gemv_dev(self, x_ptr: int, y_ptr: int, rows: int, stream=None):
+        """y[rows, N] = x[rows, K] . dequant(W), device pointers."""
+        check(self.ctx.L.shainet_attn_q4_gemv_dev(self.ctx.h, self.h, x_ptr, y_ptr, rows, _stream_arg(stream)))
+
+    def close(self):
+        if getattr(self, "h", None):
+            check(self.ctx.L.shainet_attn_q4_destroy(self.h))
             self.h = None
 
 

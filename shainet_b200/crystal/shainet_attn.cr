@@ -123,6 +123,41 @@ module SHAInet
                                                      start_pos : Int32, num_heads : Int32, heads_per_kv : Int32,
                                                      head_dim : Int32, capacity : Int32, scale : Float32,
                                                      stream : Void*) : Int32
+
+    # keys and values of many requests in pages of one pool
+    type Paged = Void*
+    fun paged_plan_dev = shainet_attn_paged_plan_dev(ctx : Ctx, requests : Int32, lens : Int32*, delta : Int32*,
+                                                     block_table : Int32*, table_width : Int32, page_rows : Int32,
+                                                     free_pages : Int32*, num_pages : Int32, free_count : Int32*,
+                                                     lens_out : Int32*, free_count_out : Int32*, first : Int32*,
+                                                     slots : Int32*, max_tokens : Int32, status : Int32*,
+                                                     stream : Void*) : Int32
+    fun paged_create = shainet_attn_paged_create(ctx : Ctx, out_paged : Paged*, num_heads : Int32, num_kv_heads : Int32,
+                                                 head_dim : Int32, page_rows : Int32, format : Int32) : Int32
+    fun paged_destroy = shainet_attn_paged_destroy(paged : Paged) : Int32
+    fun paged_decode_dev = shainet_attn_paged_decode_dev(ctx : Ctx, paged : Paged, kv : Kv, k_pages : Void*, v_pages : Void*,
+                                                         num_pages : Int32, q : Float32*, k_new : Float32*, v_new : Float32*,
+                                                         out_ptr : Float32*, block_table : Int32*, table_width : Int32,
+                                                         lens : Int32*, requests : Int32, scale : Float32,
+                                                         stream : Void*) : Int32
+    fun paged_scatter_dev = shainet_attn_paged_scatter_dev(ctx : Ctx, paged : Paged, kv : Kv, k_pages : Void*, v_pages : Void*,
+                                                           num_pages : Int32, slots : Int32*, row0 : Int32, rows : Int32,
+                                                           stream : Void*) : Int32
+    fun paged_gather_dev = shainet_attn_paged_gather_dev(ctx : Ctx, paged : Paged, kv : Kv, k_pages : Void*, v_pages : Void*,
+                                                         num_pages : Int32, table_row : Int32*, rows : Int32,
+                                                         stream : Void*) : Int32
+
+    # 4-bit weights with group scales
+    type Q4 = Void*
+    fun q4_create = shainet_attn_q4_create(ctx : Ctx, out_w : Q4*, w_host : Float32*, k : Int32, n : Int32, group : Int32) : Int32
+    fun q4_create_raw = shainet_attn_q4_create_raw(ctx : Ctx, out_w : Q4*, packed_host : UInt8*, scales_host : Float32*,
+                                                   k : Int32, n : Int32, group : Int32) : Int32
+    fun q4_create_dev = shainet_attn_q4_create_dev(ctx : Ctx, out_w : Q4*, packed_dev : UInt8*, scales_dev : Float32*,
+                                                   k : Int32, n : Int32, group : Int32) : Int32
+    fun q4_destroy = shainet_attn_q4_destroy(w : Q4) : Int32
+    fun q4_export = shainet_attn_q4_export(w : Q4, packed_host : UInt8*, scales_host : Float32*) : Int32
+    fun q4_gemv_dev = shainet_attn_q4_gemv_dev(ctx : Ctx, w : Q4, x_dev : Float32*, y_dev : Float32*, rows : Int32,
+                                               stream : Void*) : Int32
   end
 
   # Thin, exception-raising wrapper in the style of SHAInet::CUDA (src/shainet/cuda.cr).

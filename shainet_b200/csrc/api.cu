@@ -189,9 +189,11 @@ int kv_ensure(shainet_attn_kv* kv, int total_len, cudaStream_t s) {
 
 int check_status(shainet_attn_ctx* ctx) {
     if (ctx->status_host && ctx->status_host->code != DEV_OK) {
-        const int where = ctx->status_host->where;
+        const int code = ctx->status_host->code, where = ctx->status_host->where;
         ctx->status_host->code = DEV_OK;
         ctx->status_host->where = 0;
+        if (code == DEV_BAD_PAGE)
+            return fail(SHAINET_ATTN_E_INVALID, "a paged call met a table cell or slot outside its pool, or a length outside its table (site %d)", where);
         if (ctx->tickets) cudaMemset(ctx->tickets, 0, ctx->tickets_cap * sizeof(unsigned));  // an unwound kernel may leave counts
         return fail(SHAINET_ATTN_E_DEVICE_WAIT, "a kernel gave up on a bounded wait (site %d)", where);
     }
@@ -572,6 +574,8 @@ int upload_vec(float*& dst, const float* host, size_t n) {
     CU(cudaMemcpy(dst, host, n * sizeof(float), cudaMemcpyHostToDevice));
     return SHAINET_ATTN_OK;
 }
+
+int kv_ensure_rows(shainet_attn_kv* kv, int rows, cudaStream_t s) { return kv_ensure(kv, rows, s); }
 
 bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
 

@@ -14,6 +14,7 @@ namespace shainet {
 enum DeviceStatus : int {
     DEV_OK = 0,
     DEV_WAIT_TIMEOUT = 1,   // an mbarrier wait ran past its time limit
+    DEV_BAD_PAGE = 2,       // a table cell, slot or length outside the pool or its table
 };
 
 struct AttnStatus {
@@ -93,6 +94,11 @@ __device__ __forceinline__ void bulk_g2s(void* smem_dst, const void* gsrc, uint3
         "cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(smem_u32(smem_dst)),
         "l"(gsrc), "r"(bytes), "r"(smem_u32(bar))
         : "memory");
+}
+
+// Records the first failure of a context for its next blocking call; the kernel carries on without the bad access.
+__device__ __forceinline__ void report_status(AttnStatus* status, int code, int where) {
+    if (status != nullptr && atomicCAS(&status->code, DEV_OK, code) == DEV_OK) status->where = where;
 }
 
 __device__ __forceinline__ float4 lds128(const float* p) { return *reinterpret_cast<const float4*>(p); }

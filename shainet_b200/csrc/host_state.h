@@ -130,6 +130,8 @@ int grow(DevBuf& b, size_t floats, cudaStream_t s);
 // dst = device copy of host[n] (allocated on first use); host == null frees it.
 int upload_vec(float*& dst, const float* host, size_t n);
 bool aligned16(const void* p);
+// Capacity for `rows` rows, by the cache's own growth policy (may allocate, move the rows and synchronise `s`).
+int kv_ensure_rows(shainet_attn_kv* kv, int rows, cudaStream_t s);
 // Norm/RoPE/append + attention of T new tokens of one sequence, device pointers, stream s.
 int forward_device(shainet_attn_ctx* ctx, shainet_attn_kv* kv, const float* q, const float* k_new, const float* v_new,
                    float* out, int T, float scale, unsigned flags, cudaStream_t s);

@@ -218,6 +218,72 @@ cudaError_t launch_embed_rows(const int* ids_dev, const float* table, float* x, 
 cudaError_t launch_argmax_decode(const unsigned long long* words, int* tokens, int n, int* next_id, int* history,
                                  int history_pos, cudaStream_t s);
 
+// One step of the block tables of `requests` requests: see shainet_attn_paged_plan_dev.
+struct PagedPlanArgs {
+    const int* lens;
+    const int* delta;
+    int* block_table;       // [requests, table_width]
+    int* free_pages;        // [num_pages], a stack of free_count[0] entries
+    const int* free_count;
+    int* lens_out;          // may be lens
+    int* free_count_out;    // may be free_count
+    int* first;             // [requests + 1]
+    int* slots;             // [max_tokens]
+    int* status;            // [2]
+    int requests, table_width, page_rows, num_pages, max_tokens;
+};
+cudaError_t launch_paged_plan(const PagedPlanArgs& a, cudaStream_t s);
+
+// One decode token for each of `requests` requests over pages: see shainet_attn_paged_decode_dev.
+struct PagedDecodeArgs {
+    void* k_pages;          // [num_pages, num_kv_heads, page_rows, head_dim]
+    void* v_pages;
+    int num_pages, page_rows;
+    const float* q;         // raw projections, [requests, num_heads*head_dim]
+    const float* k_new;     // [requests, num_kv_heads*head_dim]
+    const float* v_new;
+    const float* b_q;       // nullable biases and per-head norm weights
+    const float* b_k;
+    const float* b_v;
+    const float* q_norm;
+    const float* k_norm;
+    const float* inv_freq;  // [head_dim/2]
+    double eps;
+    float* out;             // [requests, num_heads*head_dim]
+    const int* block_table; // [requests, table_width]
+    int table_width;
+    const int* lens;        // [requests], the new token included; 0: a padded row
+    int requests;
+    HeadShape hs;
+    float scale;
+    int kv_elem_bytes;
+    AttnStatus* status;
+};
+cudaError_t launch_paged_decode(const PagedDecodeArgs& a, cudaStream_t s);
+
+// Rows [row0, row0 + rows) of a cache to the slots `index` (scatter), or rows [0, rows) of the pages of the table row
+// `index` into the cache (gather, row0 = 0).  row_bytes is 128, 256 or 512.
+struct PagedCopyArgs {
+    void* k_pages;
+    void* v_pages;
+    void* k_cache;          // [num_kv_heads, capacity, head_dim]
+    void* v_cache;
+    const int* index;
+    int num_pages, page_rows, num_kv_heads, capacity, row0, rows, row_bytes;
+    AttnStatus* status;
+};
+cudaError_t launch_paged_copy(const PagedCopyArgs& a, bool scatter, cudaStream_t s);
+
+// y[M, N] = x[M, K] . dequant(W) over 4-bit weights in the layout of q4_gemv.cu.
+struct Q4GemvArgs {
+    const float* x;
+    const uint4* q;
+    const float* scales;
+    float* y;
+    int M, N, K, group;
+};
+cudaError_t launch_q4_gemv(const Q4GemvArgs& a, int sm_count, cudaStream_t s);
+
 // Sets the calling thread's message for shainet_attn_last_error().
 void set_last_error_message(const char* msg);
 

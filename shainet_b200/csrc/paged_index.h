@@ -1,0 +1,36 @@
+// Index arithmetic of paged caches, shared by the kernels and the host (plain C++: it also compiles without nvcc).
+//
+// A pool holds num_pages pages of [num_kv_heads, page_rows, head_dim] elements per tensor; a block table row lists the
+// pages of a request in the order of its positions.
+#pragma once
+#include <stddef.h>
+
+#ifdef __CUDACC__
+#define SHAINET_HD __host__ __device__ __forceinline__
+#else
+#define SHAINET_HD inline
+#endif
+
+namespace shainet {
+
+constexpr int PAGED_MAX_PAGE_ROWS = 4096;
+
+SHAINET_HD int pages_for(long long positions, int page_rows) { return (int)((positions + page_rows - 1) / page_rows); }
+
+// A table cell is followed, and a slot used, only where it lies in the pool.
+SHAINET_HD bool page_in_pool(int page, int num_pages) { return page >= 0 && page < num_pages; }
+SHAINET_HD bool slot_in_pool(int slot, int num_pages, int page_rows) {
+    return slot >= 0 && slot < (long long)num_pages * page_rows;
+}
+
+// A length that a table row can hold; anything else is an empty request.
+SHAINET_HD bool length_fits(int len, int table_width, int page_rows) {
+    return len >= 0 && len <= (long long)table_width * page_rows;
+}
+
+// Row of a tensor's pool, in units of head_dim elements: 64 bits, a pool may hold more than 2^31 elements.
+SHAINET_HD size_t pool_row(int page, int num_kv_heads, int kv_head, int page_rows, int row) {
+    return ((size_t)page * num_kv_heads + kv_head) * page_rows + row;
+}
+
+}  // namespace shainet

@@ -1,0 +1,191 @@
+// Block tables and slot maps of a batch of requests, built on the device from the requests' lengths, sm_100a.
+//
+// Per request r with length l, change d and pages of P rows: before = ceil(l / P), after = ceil((l + d) / P); the request
+// grows by max(after - before, 0) pages, frees max(before - after, 0) and has max(d, 0) new tokens.  Exclusive sums of
+// the three over the requests give every page that moves and every token its place, so after one scan all cells of the
+// outputs are independent: the i-th page a request grows by is entry f + freed - 1 - i of the stack that the f free
+// pages and the freed ones behind them form; the page of a new token comes from the request's old table row or, by the
+// same index, from the stack.  A freed page that is popped again in the same step is looked up in the table row that
+// frees it, never in the stack cell that is being written, so nothing waits for a write of this launch.
+//
+// What bounds it is latency, not bytes (a few hundred KB at most): one round of loads, a scan over at most 8192 requests
+// that every CTA does for itself in shared memory, one or two dependent loads per output.  Large steps are spread over
+// one cluster of eight CTAs, whose barrier separates the reads of lens and free_count from the writes of lens_out and
+// free_count_out, which may be the same arrays; small ones take one CTA.
+#include "kernels.h"
+#include "paged_index.h"
+
+namespace shainet {
+
+namespace {
+
+constexpr int PLAN_THREADS = 1024;
+constexpr int PLAN_WARPS = PLAN_THREADS / 32;
+constexpr int PLAN_CLUSTER = 8;
+constexpr unsigned FULL = 0xffffffffu;
+enum PlanStatus { PLAN_OK = 0, PLAN_SHORT = 1, PLAN_LENGTH = 2, PLAN_TOKENS = 3, PLAN_STACK = 4 };
+
+struct Sums {
+    long long tokens;
+    int grow, shrink;
+};
+
+__device__ __forceinline__ Sums operator+(Sums a, Sums b) { return {a.tokens + b.tokens, a.grow + b.grow, a.shrink + b.shrink}; }
+
+__device__ __forceinline__ Sums shfl_up(Sums v, int off) {
+    return {__shfl_up_sync(FULL, v.tokens, off), __shfl_up_sync(FULL, v.grow, off), __shfl_up_sync(FULL, v.shrink, off)};
+}
+
+// The last r with sums[r] <= x (sums is non-decreasing, sums[0] == 0): the request that owns element x.
+__device__ __forceinline__ int owner_of(const int* sums, int n, int x) {
+    int lo = 0, hi = n - 1;
+    while (lo < hi) {
+        const int mid = (lo + hi + 1) >> 1;
+        if (sums[mid] <= x) lo = mid;
+        else hi = mid - 1;
+    }
+    return lo;
+}
+
+__device__ __forceinline__ Sums change_of(int len, int delta, int page_rows) {
+    const int before = pages_for(len, page_rows), after = pages_for((long long)len + delta, page_rows);
+    return {delta > 0 ? delta : 0, after > before ? after - before : 0, before > after ? before - after : 0};
+}
+
+__global__ void __launch_bounds__(PLAN_THREADS) paged_plan_kernel(PagedPlanArgs a) {
+    extern __shared__ int plan_smem[];
+    const int R = a.requests, P = a.page_rows;
+    int* s_len = plan_smem;
+    int* s_delta = s_len + R;
+    int* s_new = s_delta + R;     // exclusive sums over the requests
+    int* s_grow = s_new + R;
+    int* s_shrink = s_grow + R;
+    __shared__ Sums warp_sums[PLAN_WARPS];
+    __shared__ int s_bad;
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    if (tid == 0) s_bad = R;
+    const int f = a.free_count[0];
+    __syncthreads();
+    for (int r = tid; r < R; r += PLAN_THREADS) {
+        const int len = a.lens[r];
+        int delta = a.delta[r];
+        const long long after = (long long)len + delta;
+        if (!length_fits(len, a.table_width, P) || after < 0 || after > (long long)a.table_width * P) {
+            atomicMin(&s_bad, r);
+            delta = 0;
+        }
+        s_len[r] = len;
+        s_delta[r] = delta;
+    }
+    __syncthreads();
+    // a thread sums a run of requests, the runs are scanned over the CTA; a length that does not fit has change 0 and
+    // ends in an error below, its page count is not used
+    const int run = (R + PLAN_THREADS - 1) / PLAN_THREADS;
+    const int r0 = min(tid * run, R), r1 = min(r0 + run, R);
+    Sums mine{0, 0, 0};
+    for (int r = r0; r < r1; ++r) mine = mine + change_of(s_len[r], s_delta[r], P);
+    Sums incl = mine;
+#pragma unroll
+    for (int off = 1; off < 32; off <<= 1) {
+        const Sums up = shfl_up(incl, off);
+        if (lane >= off) incl = incl + up;
+    }
+    if (lane == 31) warp_sums[warp] = incl;
+    __syncthreads();
+    Sums base{0, 0, 0}, total{0, 0, 0};
+    for (int w = 0; w < PLAN_WARPS; ++w) {
+        if (w == warp) base = total;
+        total = total + warp_sums[w];
+    }
+    Sums at{base.tokens + incl.tokens - mine.tokens, base.grow + incl.grow - mine.grow, base.shrink + incl.shrink - mine.shrink};
+    for (int r = r0; r < r1; ++r) {
+        s_new[r] = (int)at.tokens;     // exact where it is used: the total is at most max_tokens
+        s_grow[r] = at.grow;
+        s_shrink[r] = at.shrink;
+        at = at + change_of(s_len[r], s_delta[r], P);
+    }
+    __syncthreads();
+    const int freed = total.shrink;
+    const long long left = (long long)f + freed - total.grow;
+    int code = PLAN_OK, detail = 0;
+    if (s_bad < R) code = PLAN_LENGTH, detail = s_bad;
+    else if (f < 0 || (long long)f + freed > a.num_pages) code = PLAN_STACK, detail = f;
+    else if (total.tokens > a.max_tokens) code = PLAN_TOKENS, detail = (int)min(total.tokens, (long long)0x7fffffff);
+    else if (left < 0) code = PLAN_SHORT, detail = (int)-left;
+
+    // every CTA has read lens and free_count before any writes lens_out and free_count_out
+    int ctas = 1, rank = 0;
+    asm("mov.u32 %0, %%cluster_nctarank;" : "=r"(ctas));
+    asm("mov.u32 %0, %%cluster_ctarank;" : "=r"(rank));
+    if (ctas > 1)
+        asm volatile("barrier.cluster.arrive.aligned;\n barrier.cluster.wait.aligned;" ::: "memory");
+
+    const int t0 = rank * PLAN_THREADS + tid, step = ctas * PLAN_THREADS;
+    const bool ok = code == PLAN_OK;
+    if (t0 == 0) {
+        a.status[0] = code;
+        a.status[1] = detail;
+        a.free_count_out[0] = ok ? (int)left : f;
+        a.first[R] = ok ? (int)total.tokens : 0;
+    }
+    for (int r = t0; r < R; r += step) {
+        a.lens_out[r] = s_len[r] + (ok ? s_delta[r] : 0);
+        a.first[r] = ok ? s_new[r] : 0;
+    }
+    if (!ok) {
+        for (int t = t0; t < a.max_tokens; t += step) a.slots[t] = -1;
+        return;
+    }
+    // the k-th freed page
+    auto freed_page = [&](int k) {
+        const int r = owner_of(s_shrink, R, k);
+        return a.block_table[(size_t)r * a.table_width + pages_for((long long)s_len[r] + s_delta[r], P) + k - s_shrink[r]];
+    };
+    // the i-th page that is popped
+    auto popped_page = [&](int i) {
+        const int at = f + freed - 1 - i;
+        return at < f ? a.free_pages[at] : freed_page(at - f);
+    };
+    for (int k = t0; k < freed; k += step) a.free_pages[f + k] = freed_page(k);
+    for (int i = t0; i < total.grow; i += step) {
+        const int r = owner_of(s_grow, R, i);
+        a.block_table[(size_t)r * a.table_width + pages_for(s_len[r], P) + i - s_grow[r]] = popped_page(i);
+    }
+    for (int t = t0; t < a.max_tokens; t += step) {
+        int slot = -1;
+        if (t < total.tokens) {
+            const int r = owner_of(s_new, R, t);
+            const long long pos = (long long)s_len[r] + t - s_new[r];
+            const int col = (int)(pos / P), before = pages_for(s_len[r], P);
+            const int page = col < before ? a.block_table[(size_t)r * a.table_width + col] : popped_page(s_grow[r] + col - before);
+            slot = (int)(page * (long long)P + pos % P);
+        }
+        a.slots[t] = slot;
+    }
+}
+
+}  // namespace
+
+cudaError_t launch_paged_plan(const PagedPlanArgs& a, cudaStream_t s) {
+    // one CTA up to 8 tokens and 2 requests a thread: a cluster's launch and barrier cost more than it saves there
+    const bool wide = a.max_tokens > 8 * PLAN_THREADS || a.requests > 2 * PLAN_THREADS;
+    const size_t smem = (size_t)a.requests * 5 * sizeof(int);
+    if (smem > 48 * 1024) {
+        cudaError_t e = cudaFuncSetAttribute(paged_plan_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+        if (e != cudaSuccess) return e;
+    }
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = dim3(wide ? PLAN_CLUSTER : 1);
+    cfg.blockDim = dim3(PLAN_THREADS);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = s;
+    cudaLaunchAttribute at[1];
+    at[0].id = cudaLaunchAttributeClusterDimension;
+    at[0].val.clusterDim.x = cfg.gridDim.x;
+    at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
+    cfg.attrs = at;
+    cfg.numAttrs = 1;
+    return cudaLaunchKernelEx(&cfg, paged_plan_kernel, a);
+}
+
+}  // namespace shainet
