@@ -98,19 +98,27 @@ def draw(rng):
 
 # ---- inputs ----
 
-class State:
-    """What the program holds.  Library objects are given back, newest first, when the state is gone."""
+class Owned:
+    """Library objects of one state, given back, newest first, when neither the state nor a tensor over their memory is
+    left."""
 
     def __init__(self):
         self.objects = []
 
-    def keep(self, obj):
-        self.objects.append(obj)
-        return obj
-
     def __del__(self):
         while self.objects:
             self.objects.pop().close()
+
+
+class State:
+    """What the program holds."""
+
+    def __init__(self):
+        self.owned = Owned()
+
+    def keep(self, obj):
+        self.owned.objects.append(obj)
+        return obj
 
 
 _ctx = None
@@ -265,7 +273,7 @@ def prepare(case, seed):
             else:
                 st.attn.cache.reserve(st.rows)
                 shape = (KV, st.attn.cache.capacity, hd)
-                st.got = [torch.as_tensor(_DeviceArray(p, shape, st.attn), device="cuda")[:, :st.rows]
+                st.got = [torch.as_tensor(_DeviceArray(p, shape, st.owned), device="cuda")[:, :st.rows]
                           for p in st.attn.cache.device_ptrs()]
     torch.cuda.synchronize()
     return st
