@@ -258,8 +258,19 @@ struct PagedDecodeArgs {
     float scale;
     int kv_elem_bytes;
     AttnStatus* status;
+    // set by the launch
+    int head_tiles;         // tiles of query heads per kv head
+    float* part_o;          // [ctas][2][gt][head_dim]: parts of (request, kv head) pairs that several CTAs share
+    float* part_ml;         // [ctas][2][gt][2]
+    unsigned* counters;     // [ctas], zero between launches
 };
-cudaError_t launch_paged_decode(const PagedDecodeArgs& a, cudaStream_t s);
+struct PagedPlan {
+    int head_tiles, gt;     // gt: query heads of a tile, rounded up to what the kernels are built for
+    int ctas;
+    size_t part_floats;
+};
+PagedPlan paged_decode_plan(const HeadShape& hs, int kv_elem_bytes, int sm_count);
+cudaError_t launch_paged_decode(PagedDecodeArgs a, const PagedPlan& p, float* workspace, unsigned* counters, cudaStream_t s);
 
 // Rows [row0, row0 + rows) of a cache to the slots `index` (scatter), or rows [0, rows) of the pages of the table row
 // `index` into the cache (gather, row0 = 0).  row_bytes is 128, 256 or 512.

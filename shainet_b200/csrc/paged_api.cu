@@ -15,6 +15,9 @@ struct shainet_attn_paged {
     HeadShape hs{};
     int page_rows = 0;
     int es = 4;
+    PagedPlan plan{};
+    float* workspace = nullptr;     // device, plan.part_floats
+    unsigned* counters = nullptr;   // device, plan.ctas, zero between calls
 };
 
 namespace {
@@ -136,13 +139,28 @@ int shainet_attn_paged_create(shainet_attn_ctx* ctx, shainet_attn_paged** out, i
     p->hs = HeadShape{num_heads, num_kv_heads, head_dim};
     p->page_rows = page_rows;
     p->es = format == SHAINET_ATTN_KV_BF16 ? 2 : 4;
+    p->plan = paged_decode_plan(p->hs, p->es, ctx->sm_count);
     ctx->live_caches++;
+    DeviceGuard g(ctx->device);
+    cudaError_t e = cudaMalloc(&p->workspace, p->plan.part_floats * sizeof(float));
+    if (e == cudaSuccess) e = cudaMalloc(&p->counters, p->plan.ctas * sizeof(unsigned));
+    if (e == cudaSuccess) e = cudaMemsetAsync(p->counters, 0, p->plan.ctas * sizeof(unsigned), ctx->stream);
+    if (e == cudaSuccess) e = cudaStreamSynchronize(ctx->stream);
+    if (e != cudaSuccess) {
+        shainet_attn_paged_destroy(p);
+        return fail_cuda(e, "workspace of a paged handle");
+    }
     *out = p;
     return SHAINET_ATTN_OK;
 }
 
 int shainet_attn_paged_destroy(shainet_attn_paged* p) {
     if (!p) return SHAINET_ATTN_OK;
+    DeviceGuard g(p->ctx->device);
+    cudaStreamSynchronize(p->ctx->stream);
+    if (p->workspace) cudaFree(p->workspace);
+    if (p->counters) cudaFree(p->counters);
+    cudaGetLastError();
     p->ctx->live_caches--;
     delete p;
     return SHAINET_ATTN_OK;
@@ -156,7 +174,6 @@ int shainet_attn_paged_decode_dev(shainet_attn_ctx* ctx, shainet_attn_paged* pag
     int rc = check_table(requests, table_width);
     if (!rc) rc = check_paged(ctx, paged, kv, k_pages, v_pages, num_pages);
     if (rc || requests == 0) return rc;
-    if (requests > 65535) return fail(SHAINET_ATTN_E_UNSUPPORTED, "%d requests: a call takes at most 65535", requests);
     if (!q || !k_new || !v_new || !out || !block_table || !lens) return fail(SHAINET_ATTN_E_INVALID, "null tensor pointer");
     if (!aligned16(q) || !aligned16(k_new) || !aligned16(v_new) || !aligned16(out))
         return fail(SHAINET_ATTN_E_INVALID, "device pointers must be 16-byte aligned");
@@ -187,7 +204,7 @@ int shainet_attn_paged_decode_dev(shainet_attn_ctx* ctx, shainet_attn_paged* pag
     a.kv_elem_bytes = paged->es;
     a.status = ctx->status_dev;
     plain_launch(ctx);
-    CU(launch_paged_decode(a, stream ? (cudaStream_t)stream : ctx->stream));
+    CU(launch_paged_decode(a, paged->plan, paged->workspace, paged->counters, stream ? (cudaStream_t)stream : ctx->stream));
     return SHAINET_ATTN_OK;
 }
 
