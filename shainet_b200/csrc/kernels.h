@@ -3,6 +3,7 @@
 #include <cuda_runtime.h>
 #include <stddef.h>
 #include "common.cuh"
+#include "paged_index.h"
 
 namespace shainet {
 
@@ -259,10 +260,11 @@ struct PagedDecodeArgs {
     int kv_elem_bytes;
     AttnStatus* status;
     // set by the launch
+    FastDiv by_page;        // division by page_rows
     int head_tiles;         // tiles of query heads per kv head
     float* part_o;          // [ctas][2][gt][head_dim]: parts of (request, kv head) pairs that several CTAs share
     float* part_ml;         // [ctas][2][gt][2]
-    unsigned* counters;     // [ctas], zero between launches
+    unsigned* counters;     // [ctas][3], zero between launches
 };
 struct PagedPlan {
     int head_tiles, gt;     // gt: query heads of a tile, rounded up to what the kernels are built for

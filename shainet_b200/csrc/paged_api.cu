@@ -17,7 +17,7 @@ struct shainet_attn_paged {
     int es = 4;
     PagedPlan plan{};
     float* workspace = nullptr;     // device, plan.part_floats
-    unsigned* counters = nullptr;   // device, plan.ctas, zero between calls
+    unsigned* counters = nullptr;   // device, 3 * plan.ctas, zero between calls
 };
 
 namespace {
@@ -49,11 +49,15 @@ int check_paged(shainet_attn_ctx* ctx, const shainet_attn_paged* paged, const sh
         return fail(SHAINET_ATTN_E_INVALID, "the cache's head layout or format is not the handle's");
     if (!k_pages || !v_pages) return fail(SHAINET_ATTN_E_INVALID, "null page pointer");
     if (!aligned16(k_pages) || !aligned16(v_pages)) return fail(SHAINET_ATTN_E_INVALID, "page pointers must be 16-byte aligned");
-    return check_pool(num_pages, paged->page_rows);
+    int rc = check_pool(num_pages, paged->page_rows);
+    if (!rc && (unsigned long long)num_pages * paged->page_rows * paged->hs.num_kv_heads > 0xfffffffeull)   // row numbers of the kernels: 32 bits
+        rc = fail(SHAINET_ATTN_E_UNSUPPORTED, "%d pages of %d rows and %d kv heads: a pool holds at most 2^32 - 2 rows of all heads", num_pages,
+                  paged->page_rows, paged->hs.num_kv_heads);
+    return rc;
 }
 
-// The calls of a paged step are ordinary launches (no programmatic serialization): they start when all work ahead of them
-// in the stream is complete, and the next kernel of the context starts behind them.
+// A paged call's kernel touches nothing before all work ahead of it in the stream is complete, and lets the next kernel
+// launch only then or at its end: a fused decode kernel behind it finds no row of a contiguous cache under construction.
 void plain_launch(shainet_attn_ctx* ctx) { ctx->last_fused = false; }
 
 int copy_rows(shainet_attn_ctx* ctx, const shainet_attn_paged* paged, const shainet_attn_kv* kv, void* k_pages, void* v_pages,
@@ -143,8 +147,8 @@ int shainet_attn_paged_create(shainet_attn_ctx* ctx, shainet_attn_paged** out, i
     ctx->live_caches++;
     DeviceGuard g(ctx->device);
     cudaError_t e = cudaMalloc(&p->workspace, p->plan.part_floats * sizeof(float));
-    if (e == cudaSuccess) e = cudaMalloc(&p->counters, p->plan.ctas * sizeof(unsigned));
-    if (e == cudaSuccess) e = cudaMemsetAsync(p->counters, 0, p->plan.ctas * sizeof(unsigned), ctx->stream);
+    if (e == cudaSuccess) e = cudaMalloc(&p->counters, 3 * p->plan.ctas * sizeof(unsigned));
+    if (e == cudaSuccess) e = cudaMemsetAsync(p->counters, 0, 3 * p->plan.ctas * sizeof(unsigned), ctx->stream);
     if (e == cudaSuccess) e = cudaStreamSynchronize(ctx->stream);
     if (e != cudaSuccess) {
         shainet_attn_paged_destroy(p);

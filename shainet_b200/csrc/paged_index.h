@@ -28,6 +28,22 @@ SHAINET_HD bool length_fits(int len, int table_width, int page_rows) {
     return len >= 0 && len <= (long long)table_width * page_rows;
 }
 
+// Quotient by page_rows without a division: n / d for 0 <= n < 2^31, 1 <= d <= 2^31 as (n * mul) >> shift, with
+// shift = 31 + ceil(log2 d) and mul = ceil(2^shift / d) (Granlund and Montgomery 1994: mul * d exceeds 2^shift by less
+// than d <= 2^(shift - 31), so the error of n * mul / 2^shift stays below 1 / d).
+struct FastDiv {
+    unsigned mul;
+    int shift;
+};
+inline FastDiv fast_div(int d) {
+    FastDiv f;
+    f.shift = 31;
+    while ((1ll << (f.shift - 31)) < d) ++f.shift;
+    f.mul = (unsigned)(((1ull << f.shift) + d - 1) / d);
+    return f;
+}
+SHAINET_HD int divide(int n, FastDiv f) { return (int)(((unsigned long long)(unsigned)n * f.mul) >> f.shift); }
+
 // Row of a tensor's pool, in units of head_dim elements: 64 bits, a pool may hold more than 2^31 elements.
 SHAINET_HD size_t pool_row(int page, int num_kv_heads, int kv_head, int page_rows, int row) {
     return ((size_t)page * num_kv_heads + kv_head) * page_rows + row;

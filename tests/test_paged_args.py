@@ -109,6 +109,15 @@ int t_pages(long long n, int p) { return pages_for(n, p); }
 int t_page(int page, int n) { return page_in_pool(page, n); }
 int t_slot(int slot, int n, int p) { return slot_in_pool(slot, n, p); }
 int t_len(int len, int w, int p) { return length_fits(len, w, p); }
+int t_div(int n, int d) { return divide(n, fast_div(d)); }
+long long t_div_sweep(int d) {      // first n whose quotient is wrong, or -1: around every multiple up to 2^31 - 1, or a grid of them
+    const FastDiv f = fast_div(d);
+    const long long step = (2147483647ll / d / 20000 + 1) * d;
+    for (long long m = 0; m <= 2147483647ll; m += step)
+        for (long long n = m - 2; n <= m + 2; ++n)
+            if (n >= 0 && n <= 2147483647ll && divide((int)n, f) != (int)(n / d)) return n;
+    return divide(2147483647, f) == 2147483647 / d ? -1 : 2147483647;
+}
 unsigned long long t_row(int page, int kv, int h, int p, int r) { return pool_row(page, kv, h, p, r); }
 }
 """
@@ -124,6 +133,8 @@ def test_index_arithmetic_keeps_bad_pages_out_and_64_bits(tmp_path):
     L = C.CDLL(str(so))
     L.t_pages.argtypes = [C.c_longlong, C.c_int]
     L.t_row.restype = C.c_ulonglong
+    L.t_div_sweep.restype = C.c_longlong
+    assert all(L.t_div_sweep(d) == -1 for d in [*range(1, 130), *range(131, 4097, 61), 4095, 4096])
     big = 2**31 - 1
     assert [L.t_pages(n, 16) for n in (0, 1, 16, 17)] == [0, 1, 1, 2] and L.t_pages(big, 1) == big
     assert [L.t_page(p, 5) for p in (-1, 0, 4, 5, big, -big)] == [0, 1, 1, 0, 0, 0]
