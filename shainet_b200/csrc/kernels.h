@@ -260,10 +260,12 @@ struct PagedDecodeArgs {
     int kv_elem_bytes;
     AttnStatus* status;
     // set by the launch
-    FastDiv by_page;        // division by page_rows
+    int max_len;            // positions a table row holds
+    FastDiv by_page, by_tiles;   // division by page_rows and by head_tiles
     int head_tiles;         // tiles of query heads per kv head
-    float* part_o;          // [ctas][2][gt][head_dim]: parts of (request, kv head) pairs that several CTAs share
-    float* part_ml;         // [ctas][2][gt][2]
+    float* part_o;          // [3 ctas][gt][head_dim]: parts of (request, kv head) pairs that several CTAs share, two a CTA,
+                            // then the sums of groups of them
+    float* part_ml;         // [3 ctas][gt][2]
     unsigned* counters;     // [ctas][3], zero between launches
 };
 struct PagedPlan {

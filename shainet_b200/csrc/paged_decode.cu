@@ -51,15 +51,11 @@ constexpr int HALF = STAGE_BYTES / 2;
 constexpr int MIN_TILES = 4;             // tiles a CTA takes at least, on average
 constexpr int PAIR_COST = 8;             // places of the line that the start and end of a pair stand for
 constexpr int CTAS_PER_SM = 2;
-constexpr int JOIN_ML = 4096;            // bytes of the rings for maxima and weight sums while parts are joined
+constexpr int LINE_PLACES = 1 << 30;        // places of the line: 8 TB of K and V, more than a device holds
 
-// 16 bytes global -> shared; the second form writes zeros where !valid (nothing is read then).
+// 16 bytes global -> shared
 __device__ __forceinline__ void copy16(uint32_t dst, const void* src) {
     asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
-}
-__device__ __forceinline__ void copy16_or_zero(uint32_t dst, const void* src, bool valid) {
-    const int n = valid ? 16 : 0;
-    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(n) : "memory");
 }
 __device__ __forceinline__ void copy_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
 template <int N>
@@ -134,48 +130,57 @@ __device__ __forceinline__ int tile_offset(int r, int c) {
 struct Cursor {
     int b, hv, j;        // request, (kv head, tile of heads), tile of the request
     int tiles, len;      // of request b
-    long long at;
-    __device__ __forceinline__ long long place() const { return at + PAIR_COST + j; }
+    int at;
+    __device__ __forceinline__ int place() const { return at + PAIR_COST + j; }
 };
 
-__device__ __forceinline__ int valid_len(const PagedDecodeArgs& a, int b) {
-    const int len = a.lens[b];
-    return length_fits(len, a.table_width, a.page_rows) ? len : 0;
-}
+// A request's length; 0 where the table cannot hold it.
+__device__ __forceinline__ int valid_len(int len, int max_len) { return (unsigned)len <= (unsigned)max_len ? len : 0; }
 template <class C>
-__device__ __forceinline__ int tiles_of(int len) { return (int)(((long long)len + C::TW - 1) / C::TW); }
+__device__ __forceinline__ int tiles_of(int len) { return (int)(((unsigned)len + C::TW - 1) / C::TW); }
 
-// n tiles further; behind the last request b is a.requests and the place past every share.
+// The first request with positions behind b, as (request, length); the number of requests where there is none.
+__device__ __noinline__ int2 next_request(const int* lens, int b, int requests, int max_len) {
+    while (++b < requests) {
+        const int len = valid_len(lens[b], max_len);
+        if (len != 0) return make_int2(b, len);
+    }
+    return make_int2(requests, 0);
+}
+
+// n tiles further; behind the last request the place is past every share.
 template <class C>
 __device__ __forceinline__ void advance(const PagedDecodeArgs& a, Cursor& c, int n) {
     c.j += n;
+#pragma unroll 1
     while (c.j >= c.tiles) {
         c.j -= c.tiles;
         c.at += PAIR_COST + c.tiles;
         if (++c.hv == a.head_tiles * a.hs.num_kv_heads) {
+            const int2 r = next_request(a.lens, c.b, a.requests, a.max_len);
             c.hv = 0;
-            do {
-                if (++c.b >= a.requests) {
-                    c.at = 0x7fffffffffffffffll - 0x100000000ll;
-                    return;
-                }
-                c.len = valid_len(a, c.b);
-            } while (c.len == 0);
+            c.b = r.x;
+            c.len = r.y;
+            if (r.y == 0) {
+                c.at = LINE_PLACES;
+                c.j = 0;
+                return;
+            }
             c.tiles = tiles_of<C>(c.len);
         }
     }
 }
 
 // Lane r finds row r of a tile: the page of the position and the row in it, then the row of the pool (of one tensor, all
-// kv heads counted: fits 32 bits), or NO_ROW: no such cached row, or a page that is not followed.
-constexpr unsigned NO_ROW = 0xffffffffu;
+// kv heads counted: fits 32 bits).  Rows that are not there (behind the cached positions, or on a page that is not followed)
+// are copied from the pool's first row: what stands there does not count.
 struct Place {
     int page, row;
 };
 template <class C>
 __device__ __forceinline__ Place lookup_page(const PagedDecodeArgs& a, const Cursor& c, int lane) {
     const int pos = c.j * C::TW + lane;
-    Place p{-1, -1};
+    Place p{0, -1};
     if (lane < C::TW && pos < c.len - 1) {               // the newest position comes from this call's inputs
         const int col = divide(pos, a.by_page);
         p.row = pos - col * a.page_rows;
@@ -184,10 +189,10 @@ __device__ __forceinline__ Place lookup_page(const PagedDecodeArgs& a, const Cur
     return p;
 }
 __device__ __forceinline__ unsigned row_of(const PagedDecodeArgs& a, int kv_h, Place p) {
-    if (p.row < 0) return NO_ROW;
+    if (p.row < 0) return 0u;
     if (!page_in_pool(p.page, a.num_pages)) {
         report_status(a.status, DEV_BAD_PAGE, 14);
-        return NO_ROW;
+        return 0u;
     }
     return ((unsigned)p.page * a.hs.num_kv_heads + kv_h) * a.page_rows + p.row;
 }
@@ -198,23 +203,12 @@ __device__ __forceinline__ void load_tile(const unsigned char* kp, const unsigne
     constexpr int RPI = 32 / C::CH;                      // rows of one warp-wide copy
     const int sub = lane / C::CH;
     const uint32_t to = stage + tile_offset<C>(sub, lane % C::CH);
-    if (__all_sync(FULL, row != NO_ROW || lane >= C::TW)) {
 #pragma unroll
-        for (int i = 0; i < C::CPT; ++i) {
-            const unsigned r = __shfl_sync(FULL, row, i * RPI + sub);
-            const uint32_t dst = (to ^ (tile_offset<C>(i * RPI, 0) & 0x70)) + i * RPI * C::ROW;
-            copy16(dst, kp + (size_t)r * C::ROW);
-            copy16(dst + HALF, vp + (size_t)r * C::ROW);
-        }
-    } else {
-#pragma unroll
-        for (int i = 0; i < C::CPT; ++i) {
-            const unsigned r = __shfl_sync(FULL, row, i * RPI + sub);
-            const uint32_t dst = (to ^ (tile_offset<C>(i * RPI, 0) & 0x70)) + i * RPI * C::ROW;
-            const size_t at = r == NO_ROW ? 0 : (size_t)r * C::ROW;
-            copy16_or_zero(dst, kp + at, r != NO_ROW);
-            copy16_or_zero(dst + HALF, vp + at, r != NO_ROW);
-        }
+    for (int i = 0; i < C::CPT; ++i) {
+        const unsigned r = __shfl_sync(FULL, row, i * RPI + sub);
+        const uint32_t dst = (to ^ (tile_offset<C>(i * RPI, 0) & 0x70)) + i * RPI * C::ROW;
+        copy16(dst, kp + (size_t)r * C::ROW);
+        copy16(dst + HALF, vp + (size_t)r * C::ROW);
     }
 }
 
@@ -528,109 +522,101 @@ struct State {
 // The weight of a part with maximum m (scores times log2 e) under a maximum of all parts; 0 for a part that saw nothing.
 __device__ __forceinline__ float part_weight(float m, float top) { return m == -INFINITY ? 0.0f : exp2f(m - top); }
 
+// (one copy of each in the kernel: its code is long, and instructions that run once per call arrive at the pace of L2)
+__device__ __noinline__ float2 angle(float position, float freq) {
+    float2 r;
+    sincosf(__fmul_rn(position, freq), &r.y, &r.x);
+    return r;
+}
+__device__ __noinline__ float inverse_rms(float mean_square, double eps) { return (float)(1.0 / sqrt((double)mean_square + eps)); }
+
 // What a segment works on.
 struct Segment {
     int b, len, kv_h, head0, heads;
     bool owns_new, stores;     // it ends with the new position; it writes the new rows into their page
 };
 
-// The rows of projections that a segment starts from, item warp + 4n for n < MAXIT: its q rows, then, where it ends with
-// the new position, the new k and the new v row.  A warp takes every fourth; lane holds columns lane + 32c.
+// The projections that a segment starts from: its q rows into qs and, where it ends with the new position, the new k and
+// v rows into xk and xv, by asynchronous copies; then bias, norm and rotation in place, in the order and with the roundings
+// of the other decode kernels, the new rows into their page too.  A warp takes every fourth row.
 template <class C>
-struct Rows {
-    static constexpr int HD = C::HD, PL = HD / 64, MAXIT = (C::GT + 2 + NW - 1) / NW;
-    float x[MAXIT][2 * PL];
-
-    __device__ __forceinline__ static bool live(const Segment& s, int it) { return it < C::GT ? it < s.heads : it < C::GT + 2 && s.owns_new; }
-
-    __device__ __forceinline__ void load(const PagedDecodeArgs& a, const Segment& s, int warp, int lane) {
-#pragma unroll
-        for (int n = 0; n < MAXIT; ++n) {
-            const int it = warp + n * NW;
-            const bool on = live(s, it);
-            const float* src = it < C::GT ? a.q + ((size_t)s.b * a.hs.num_heads + s.head0 + it) * HD
-                                          : (it == C::GT ? a.k_new : a.v_new) + ((size_t)s.b * a.hs.num_kv_heads + s.kv_h) * HD;
-#pragma unroll
-            for (int c = 0; c < 2 * PL; ++c) x[n][c] = on ? __ldcg(src + lane + 32 * c) : 0.0f;
-        }
+__device__ __forceinline__ void request_rows(const PagedDecodeArgs& a, const Segment& s, float* qs, float* xk, float* xv, int warp, int lane) {
+    constexpr int HD = C::HD;
+    const int items = s.heads + (s.owns_new ? 2 : 0);
+#pragma unroll 1
+    for (int it = warp; it < items; it += NW) {
+        const bool is_q = it < s.heads, is_k = it == s.heads;
+        const float* src = is_q ? a.q + ((size_t)s.b * a.hs.num_heads + s.head0 + it) * HD : (is_k ? a.k_new : a.v_new) + ((size_t)s.b * a.hs.num_kv_heads + s.kv_h) * HD;
+        float* to = is_q ? qs + it * C::QS : is_k ? xk : xv;
+        if (lane < HD / 4) copy16(smem_u32(to + lane * 4), src + lane * 4);
     }
-
-    // Bias, norm and rotation, in the order and with the roundings of the other decode kernels; q rows into qs, the new
-    // rows into xk and xv and into their page.
-    __device__ __forceinline__ void finish(const PagedDecodeArgs& a, const Segment& s, float* qs, float* xk, float* xv, int warp, int lane) {
-        const int KV = a.hs.num_kv_heads, pos = s.len - 1;
-        if (a.b_q != nullptr || a.b_k != nullptr || a.b_v != nullptr) {
+}
+template <class C>
+__device__ __forceinline__ void prepare_rows(const PagedDecodeArgs& a, const Segment& s, float* qs, float* xk, float* xv, int warp, int lane) {
+    constexpr int HD = C::HD, PL = HD / 64;
+    const int pos = s.len - 1, items = s.heads + (s.owns_new ? 2 : 0);
+    float2 turn[PL];
 #pragma unroll
-            for (int n = 0; n < MAXIT; ++n) {
-                const int it = warp + n * NW;
-                const float* bias = it < C::GT ? a.b_q : it == C::GT ? a.b_k : a.b_v;
-                if (bias == nullptr || !live(s, it)) continue;
-                bias += (size_t)(it < C::GT ? s.head0 + it : s.kv_h) * HD;
+    for (int k = 0; k < PL; ++k) turn[k] = angle((float)pos, __ldg(a.inv_freq + lane + 32 * k));
+    size_t at = 0;
+    bool stores = s.owns_new && s.stores;
+    if (stores) {
+        const int col = divide(pos, a.by_page), page = a.block_table[(size_t)s.b * a.table_width + col];
+        stores = page_in_pool(page, a.num_pages);
+        if (stores) at = pool_row(page, a.hs.num_kv_heads, s.kv_h, a.page_rows, pos - col * a.page_rows) * HD;
+        else if (warp == 0 && lane == 0) report_status(a.status, DEV_BAD_PAGE, 15);
+    }
+#pragma unroll 1
+    for (int it = warp; it < items; it += NW) {      // the rows this warp requested
+        const bool is_q = it < s.heads, is_k = it == s.heads;
+        float* row = is_q ? qs + it * C::QS : is_k ? xk : xv;
+        const float* bias = is_q ? a.b_q : is_k ? a.b_k : a.b_v;
+        const float* w = is_q ? a.q_norm : is_k ? a.k_norm : nullptr;
+        float x[2 * PL];
 #pragma unroll
-                for (int c = 0; c < 2 * PL; ++c) x[n][c] = __fadd_rn(x[n][c], __ldg(bias + lane + 32 * c));
+        for (int c = 0; c < 2 * PL; ++c) x[c] = row[lane + 32 * c];
+        if (bias) {
+            bias += (size_t)(is_q ? s.head0 + it : s.kv_h) * HD;
+#pragma unroll
+            for (int c = 0; c < 2 * PL; ++c) x[c] = __fadd_rn(x[c], __ldg(bias + lane + 32 * c));
+        }
+        if (w) {
+            float ss = 0.0f;
+#pragma unroll
+            for (int c = 0; c < 2 * PL; ++c) ss = fmaf(x[c], x[c], ss);
+#pragma unroll
+            for (int off = 16; off > 0; off >>= 1) ss += __shfl_xor_sync(FULL, ss, off);
+            const float inv = inverse_rms(ss / (float)HD, a.eps);
+#pragma unroll
+            for (int c = 0; c < 2 * PL; ++c) x[c] = __fmul_rn(__fmul_rn(x[c], inv), __ldg(w + lane + 32 * c));
+        }
+        if (is_q || is_k) {
+#pragma unroll
+            for (int k = 0; k < PL; ++k) {
+                const float x0 = x[k], x1 = x[k + PL];
+                x[k] = __fsub_rn(__fmul_rn(x0, turn[k].x), __fmul_rn(x1, turn[k].y));
+                x[k + PL] = __fadd_rn(__fmul_rn(x1, turn[k].x), __fmul_rn(x0, turn[k].y));
             }
         }
-        float rs[PL], rc[PL];
 #pragma unroll
-        for (int k = 0; k < PL; ++k) sincosf(__fmul_rn((float)pos, __ldg(a.inv_freq + lane + 32 * k)), &rs[k], &rc[k]);
-        float inv[MAXIT];
-        if (a.q_norm != nullptr || a.k_norm != nullptr) {
-#pragma unroll
-            for (int n = 0; n < MAXIT; ++n) {
-                inv[n] = 0.0f;
-#pragma unroll
-                for (int c = 0; c < 2 * PL; ++c) inv[n] = fmaf(x[n][c], x[n][c], inv[n]);
-            }
-#pragma unroll
-            for (int off = 16; off > 0; off >>= 1)
-#pragma unroll
-                for (int n = 0; n < MAXIT; ++n) inv[n] += __shfl_xor_sync(FULL, inv[n], off);
-#pragma unroll
-            for (int n = 0; n < MAXIT; ++n) inv[n] = (float)(1.0 / sqrt((double)(inv[n] / (float)HD) + a.eps));
-        }
-        bool stores = s.owns_new && s.stores;
-        int page = 0;
-        if (stores) {
-            page = a.block_table[(size_t)s.b * a.table_width + pos / a.page_rows];
-            if (!page_in_pool(page, a.num_pages)) {
-                if (warp == 0 && lane == 0) report_status(a.status, DEV_BAD_PAGE, 15);
-                stores = false;
-                page = 0;
-            }
-        }
-        const size_t at = pool_row(page, KV, s.kv_h, a.page_rows, pos % a.page_rows) * HD;
-#pragma unroll
-        for (int n = 0; n < MAXIT; ++n) {
-            const int it = warp + n * NW;
-            if (it >= C::GT + (s.owns_new ? 2 : 0)) break;
-            float* to = it < C::GT ? qs + it * C::QS : it == C::GT ? xk : xv;
-            if (it <= C::GT) {
-                const float* w = it < C::GT ? a.q_norm : a.k_norm;
-#pragma unroll
-                for (int k = 0; k < PL; ++k) {
-                    float x0 = x[n][k], x1 = x[n][k + PL];
-                    if (w) {
-                        x0 = __fmul_rn(__fmul_rn(x0, inv[n]), __ldg(w + lane + 32 * k));
-                        x1 = __fmul_rn(__fmul_rn(x1, inv[n]), __ldg(w + lane + 32 * k + HD / 2));
-                    }
-                    x[n][k] = __fsub_rn(__fmul_rn(x0, rc[k]), __fmul_rn(x1, rs[k]));
-                    x[n][k + PL] = __fadd_rn(__fmul_rn(x1, rc[k]), __fmul_rn(x0, rs[k]));
-                }
-            }
+        for (int c = 0; c < 2 * PL; ++c) row[lane + 32 * c] = x[c];
+        if (!is_q && stores) {
+            void* dst = is_k ? a.k_pages : a.v_pages;
 #pragma unroll
             for (int c = 0; c < 2 * PL; ++c) {
-                to[lane + 32 * c] = x[n][c];
-                if (it >= C::GT && stores) {
-                    void* dst = it == C::GT ? a.k_pages : a.v_pages;
-                    if constexpr (C::ES == 4) static_cast<float*>(dst)[at + lane + 32 * c] = x[n][c];
-                    else static_cast<__nv_bfloat16*>(dst)[at + lane + 32 * c] = __float2bfloat16_rn(x[n][c]);
-                }
+                if constexpr (C::ES == 4) static_cast<float*>(dst)[at + lane + 32 * c] = x[c];
+                else static_cast<__nv_bfloat16*>(dst)[at + lane + 32 * c] = __float2bfloat16_rn(x[c]);
             }
         }
     }
-};
+#pragma unroll 1
+    for (int it = s.heads + warp; it < C::GT; it += NW)      // heads that fill up the tile
+#pragma unroll
+        for (int c = 0; c < 2 * PL; ++c) qs[it * C::QS + lane + 32 * c] = 0.0f;
+}
 
-// The new k and v rows into row r of a tile, as the pages hold them.
+// The last tile of a request: the new k and v rows, as the pages hold them, into row r; v rows behind it are zeros (their
+// weights are, but what was copied there may not be finite).
 template <class C>
 __device__ __forceinline__ void patch_tile(unsigned char* st, int r, const float* xk, const float* xv, int lane) {
 #pragma unroll
@@ -644,139 +630,153 @@ __device__ __forceinline__ void patch_tile(unsigned char* st, int r, const float
             *reinterpret_cast<__nv_bfloat16*>(st + HALF + at) = __float2bfloat16_rn(xv[d]);
         }
     }
+#pragma unroll 1
+    for (int i = (r + 1) * C::CH + lane; i < C::TW * C::CH; i += 32) *reinterpret_cast<uint4*>(st + HALF + i * 16) = make_uint4(0u, 0u, 0u, 0u);
     __syncwarp();
 }
 
-// A pair that several CTAs share: parts c0 .. c0 + n - 1, the first of them its CTA's second (shift) or first.
+// A pair that several CTAs share: the parts of CTAs c0 .. c0 + n - 1.  A CTA has two places for parts: of a pair that
+// began before it (0) and of one that begins in it (1).
 struct Shared {
-    int c0, n, shift, heads;
-    bool mine;
+    int c0, n, fan, heads;     // fan: parts that are joined at once
+    bool mine;                 // this CTA joins
     float* out;
-    // Parts that are joined at once: all, where they fit the rings, or about the root of their number; then each group's
-    // last CTA joins it into the place of its first part, and the last group's joins the groups.
-    template <class C>
-    __device__ __forceinline__ int fan() const {
-        return n * heads <= ((int)C::RING - JOIN_ML) / (C::HD * 4) ? n : (int)ceilf(sqrtf((float)n));
-    }
 };
 
-// Parts staged in shared memory and added: four columns of TPT heads a thread; where the heads leave threads over, up to
-// four threads share a column's parts.
+// Parts added from the workspace: staged in the rings by asynchronous copies, all requested before the first is waited
+// for, then four columns of TPT heads a thread; where the heads leave threads over, up to four threads share a column's
+// parts.  Loops and not unrolled code: a CTA works alone here, once a call, and cold instructions arrive more slowly than
+// they are executed.
 template <class C>
 struct Join {
-    static constexpr int HD = C::HD, GT = C::GT, TPT = (GT * HD / 4 + THREADS - 1) / THREADS;
-    static constexpr int MOST = ((int)C::RING - JOIN_ML) / (HD * 4);               // (part, head) pairs that are staged at once
-    static constexpr int MLT = MOST / THREADS + 1;                                 // of them a thread brings the maxima of
-    static_assert(MOST * 8 + GT * 16 <= JOIN_ML, "maxima, weight sums and rescaling factors");
+    static constexpr int HD = C::HD, GT = C::GT, TPT = (GT * HD / 4 + THREADS - 1) / THREADS, HPW = GT / NW;
+    static constexpr int MOST = 64;                          // parts of one call; a lane brings the maxima of two a head
+    static constexpr int META = GT * 8 + MOST * GT * 4;      // bytes: sums, then weights [part][head]
+    static constexpr int SHARES = THREADS * 16;
     float4 acc[TPT];
 
-    __device__ __forceinline__ static float2* sums(unsigned char* smem) { return reinterpret_cast<float2*>(smem + C::RING - JOIN_ML) + MOST; }
+    __device__ __forceinline__ static int groups_of(int heads) {
+        const int tasks = heads * (HD / 4);
+        return tasks <= THREADS / 4 ? 4 : tasks <= THREADS / 2 ? 2 : 1;
+    }
+    // All parts at once where they fit; more in groups of about the root of their number, each by its last CTA into a second
+    // table, then the groups.
+    __device__ __forceinline__ static int fan_of(int n, int heads) {
+        return n <= MOST && n * heads * HD * 4 <= (int)C::RING - META - SHARES ? n : (int)ceilf(sqrtf((float)n));
+    }
+    static_assert(GT % NW == 0, "a warp weighs the parts of every fourth head");
 
-    // parts from, from + stride, ... (n of them); maxima and weight sums of the heads in sums()
-    __device__ __forceinline__ void run(const PagedDecodeArgs& a, const Shared& p, int from, int stride, int n, unsigned char* smem, int tid) {
+    __device__ __forceinline__ static float2* sums(unsigned char* smem) { return reinterpret_cast<float2*>(smem); }
+
+    // n parts at places at0, at0 + step, ...; the first one place further where `odd`.  Maxima and weight sums in sums().
+    __device__ __forceinline__ void run(const float* po, const float2* pml, int at0, int step, int n, int odd, int heads, unsigned char* smem, int tid) {
         const int warp = tid >> 5, lane = tid & 31;
-        const int tasks = p.heads * (HD / 4), room = MOST / p.heads;
-        const int groups = tasks <= THREADS / 4 ? 4 : tasks <= THREADS / 2 ? 2 : 1, wide = THREADS / groups, sub = tid / wide;
-        float2* ml = reinterpret_cast<float2*>(smem + C::RING - JOIN_ML);
-        float2* total = sums(smem);                                                // (maximum, weight sum) of a head
-        float* factor = reinterpret_cast<float*>(total + GT);                      // of what was summed before
+        const int tasks = heads * (HD / 4), groups = groups_of(heads), wide = THREADS / groups, sub = tid / wide, e0 = tid - sub * wide;
+        float2* total = sums(smem);
+        float* weight = reinterpret_cast<float*>(total + GT);
+        float4* share = reinterpret_cast<float4*>(smem + META);
+        unsigned char* stage = smem + META + SHARES;
+        const int room = ((int)C::RING - META - SHARES) / (tasks * 16);
+        float2 ml[HPW][2];
 #pragma unroll
-        for (int k = 0; k < TPT; ++k) acc[k] = make_float4(0.f, 0.f, 0.f, 0.f);
-        for (int i0 = 0; i0 < n; i0 += room) {
-            const int cnt = min(room, n - i0);
-            __syncthreads();
-            auto part_of = [&](int i) {
-                const int c = from + (i0 + i) * stride;
-                return (unsigned)(c * 2 + (c == p.c0 ? p.shift : 0)) * GT;
-            };
-            // all of it requested before any is waited for (L2: other SMs wrote it)
-            float2 w[MLT];
+        for (int x = 0; x < HPW; ++x)
 #pragma unroll
-            for (int k = 0; k < MLT; ++k) {
-                const int x = tid + k * THREADS;
-                if (x < cnt * p.heads) w[k] = __ldcg(reinterpret_cast<const float2*>(a.part_ml) + part_of(x / p.heads) + x % p.heads);
+            for (int k = 0; k < 2; ++k) {
+                const int g = warp + x * NW, i = lane + 32 * k;
+                ml[x][k] = make_float2(-INFINITY, 0.f);
+                if (g < heads && i < n) ml[x][k] = __ldcg(pml + (at0 + i * step + (i == 0 ? odd : 0)) * GT + g);
             }
+        auto request = [&](int i0, int cnt) {
+            const float* src = po + (size_t)((at0 + (i0 + sub) * step) * (GT * HD)) + e0 * 4;
+            uint32_t to = smem_u32(stage) + (sub * tasks + e0) * 16;
+            int skip = i0 + sub == 0 ? odd * (GT * HD) : 0;
+#pragma unroll 1
             for (int i = sub; i < cnt; i += groups) {
-                const float* from_part = a.part_o + (size_t)part_of(i) * HD;
-                for (int e = tid - sub * wide; e < tasks; e += wide) copy16(smem_u32(smem) + (i * tasks + e) * 16, from_part + e * 4);
+#pragma unroll
+                for (int x = 0; x < TPT; ++x)
+                    if (e0 + x * THREADS < tasks) copy16(to + x * (THREADS * 16), src + skip + x * (THREADS * 4));
+                skip = 0;
+                src += groups * step * (GT * HD);
+                to += groups * tasks * 16;
             }
             copy_commit();
+        };
+        int cnt = min(n, room);
+        request(0, cnt);
 #pragma unroll
-            for (int k = 0; k < MLT; ++k)
-                if (tid + k * THREADS < cnt * p.heads) ml[tid + k * THREADS] = w[k];
-            __syncthreads();
-            // maxima to weights, a warp to a head
-            for (int g = warp; g < p.heads; g += NW) {
-                const float2 old = i0 > 0 ? total[g] : make_float2(-INFINITY, 0.f);
-                float top = old.x, L = 0.0f;
-                for (int i = lane; i < cnt; i += 32) top = fmaxf(top, ml[i * p.heads + g].x);
+        for (int x = 0; x < HPW; ++x) {
+            const int g = warp + x * NW;
+            float top = fmaxf(ml[x][0].x, ml[x][1].x);
 #pragma unroll
-                for (int off = 16; off > 0; off >>= 1) top = fmaxf(top, __shfl_xor_sync(FULL, top, off));
-                for (int i = lane; i < cnt; i += 32) {
-                    const float2 x = ml[i * p.heads + g];
-                    const float wt = part_weight(x.x, top);
-                    L = fmaf(wt, x.y, L);
-                    ml[i * p.heads + g].x = wt;
-                }
+            for (int off = 16; off > 0; off >>= 1) top = fmaxf(top, __shfl_xor_sync(FULL, top, off));
+            const float w0 = part_weight(ml[x][0].x, top), w1 = part_weight(ml[x][1].x, top);
+            float L = fmaf(w0, ml[x][0].y, w1 * ml[x][1].y);
 #pragma unroll
-                for (int off = 16; off > 0; off >>= 1) L += __shfl_xor_sync(FULL, L, off);
-                __syncwarp();
-                if (lane == 0) {
-                    const float f = part_weight(old.x, top);
-                    factor[g] = f;
-                    total[g] = make_float2(top, fmaf(f, old.y, L));
-                }
+            for (int off = 16; off > 0; off >>= 1) L += __shfl_xor_sync(FULL, L, off);
+            if (g < heads) {
+                if (lane < n) weight[lane * heads + g] = w0;
+                if (lane + 32 < n) weight[(lane + 32) * heads + g] = w1;
+                if (lane == 0) total[g] = make_float2(top, L);
             }
+        }
+#pragma unroll
+        for (int x = 0; x < TPT; ++x) acc[x] = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 1
+        for (int i0 = 0;;) {
             copy_wait<0>();
             __syncthreads();
 #pragma unroll
-            for (int k = 0; k < TPT; ++k) {
-                const int e = tid - sub * wide + k * THREADS;
-                if (e >= tasks) break;
-                const int g = e / (HD / 4);
-                const float f = factor[g];
-                acc[k].x *= f, acc[k].y *= f, acc[k].z *= f, acc[k].w *= f;
+            for (int x = 0; x < TPT; ++x) {
+                const int e = e0 + x * THREADS;
+                if (e < tasks) {
+                    const float* w = weight + (i0 + sub) * heads + e / (HD / 4);
+                    const float4* v = reinterpret_cast<const float4*>(stage) + sub * tasks + e;
 #pragma unroll 4
-                for (int i = sub; i < cnt; i += groups) {
-                    const float wt = ml[i * p.heads + g].x;
-                    const float4 v = *reinterpret_cast<const float4*>(smem + (i * tasks + e) * 16);
-                    acc[k].x = fmaf(wt, v.x, acc[k].x);
-                    acc[k].y = fmaf(wt, v.y, acc[k].y);
-                    acc[k].z = fmaf(wt, v.z, acc[k].z);
-                    acc[k].w = fmaf(wt, v.w, acc[k].w);
+                    for (int i = sub; i < cnt; i += groups) {
+                        const float wt = *w;
+                        const float4 y = *v;
+                        acc[x].x = fmaf(wt, y.x, acc[x].x);
+                        acc[x].y = fmaf(wt, y.y, acc[x].y);
+                        acc[x].z = fmaf(wt, y.z, acc[x].z);
+                        acc[x].w = fmaf(wt, y.w, acc[x].w);
+                        w += groups * heads;
+                        v += groups * tasks;
+                    }
                 }
             }
+            i0 += cnt;
+            if (i0 >= n) break;
+            __syncthreads();
+            cnt = min(n - i0, room);
+            request(i0, cnt);
         }
         if (groups > 1) {        // one task a thread
-            __syncthreads();
-            float4* part = reinterpret_cast<float4*>(smem);
-            part[tid] = acc[0];
+            share[tid] = acc[0];
             __syncthreads();
             if (sub == 0)
+#pragma unroll 1
                 for (int k = 1; k < groups; ++k) {
-                    const float4 v = part[tid + k * wide];
-                    acc[0].x += v.x, acc[0].y += v.y, acc[0].z += v.z, acc[0].w += v.w;
+                    const float4 o = share[tid + k * wide];
+                    acc[0].x += o.x, acc[0].y += o.y, acc[0].z += o.z, acc[0].w += o.w;
                 }
         }
     }
-    // as the part of CTA c
-    __device__ __forceinline__ void store(const PagedDecodeArgs& a, const Shared& p, int c, unsigned char* smem, int tid) {
-        const size_t part = (size_t)(c * 2 + (c == p.c0 ? p.shift : 0)) * GT;
+    __device__ __forceinline__ void store(float* po, float2* pml, int at, int heads, unsigned char* smem, int tid) {
 #pragma unroll
-        for (int k = 0; k < TPT; ++k) {
-            const int e = tid + k * THREADS;
-            if (e >= p.heads * (HD / 4)) break;
-            *reinterpret_cast<float4*>(a.part_o + part * HD + e * 4) = acc[k];
+        for (int x = 0; x < TPT; ++x) {
+            const int e = tid + x * THREADS;
+            if (e < heads * (HD / 4)) *(reinterpret_cast<float4*>(po) + at * (GT * HD / 4) + e) = acc[x];
         }
-        if (tid < p.heads) *reinterpret_cast<float2*>(a.part_ml + (part + tid) * 2) = sums(smem)[tid];
+        if (tid < heads) pml[at * GT + tid] = sums(smem)[tid];
     }
-    __device__ __forceinline__ void finish(const Shared& p, unsigned char* smem, int tid) {
+    __device__ __forceinline__ void finish(float* out, int heads, unsigned char* smem, int tid) {
 #pragma unroll
-        for (int k = 0; k < TPT; ++k) {
-            const int e = tid + k * THREADS;
-            if (e >= p.heads * (HD / 4)) break;
-            const float inv = 1.0f / sums(smem)[e / (HD / 4)].y;
-            *reinterpret_cast<float4*>(p.out + e * 4) = make_float4(acc[k].x * inv, acc[k].y * inv, acc[k].z * inv, acc[k].w * inv);
+        for (int x = 0; x < TPT; ++x) {
+            const int e = tid + x * THREADS;
+            if (e < heads * (HD / 4)) {
+                const float inv = 1.0f / sums(smem)[e / (HD / 4)].y;
+                *reinterpret_cast<float4*>(out + e * 4) = make_float4(acc[x].x * inv, acc[x].y * inv, acc[x].z * inv, acc[x].w * inv);
+            }
         }
     }
 };
@@ -803,61 +803,71 @@ __global__ void __launch_bounds__(THREADS, CTAS_PER_SM) paged_decode_kernel(Page
     // ---- the line: its length, then the request in which this CTA's share starts.  Every warp for itself, 128 requests
     // at a time, EACH a lane ----
     int lens[EACH];
-    auto places = [&](int len) { return len > 0 ? (long long)(tiles_of<C>(len) + PAIR_COST) * HV : 0ll; };
-    auto scan = [&](int b0, long long& upto) {       // places of this lane's requests and all before them
+    auto places = [&](int len) { return len > 0 ? (tiles_of<C>(len) + PAIR_COST) * HV : 0; };
+    auto scan = [&](int b0, int& upto) {             // places of this lane's requests and all before them
 #pragma unroll
         for (int i = 0; i < EACH; ++i) {
             const int b = b0 + lane * EACH + i;
-            lens[i] = b < a.requests ? valid_len(a, b) : 0;
+            lens[i] = b < a.requests ? valid_len(a.lens[b], a.max_len) : 0;
         }
         upto = 0;
 #pragma unroll
         for (int i = 0; i < EACH; ++i) upto += places(lens[i]);
 #pragma unroll
         for (int off = 1; off < 32; off <<= 1) {
-            const long long up = __shfl_up_sync(FULL, upto, off);
+            const int up = __shfl_up_sync(FULL, upto, off);
             if (lane >= off) upto += up;
         }
         return __shfl_sync(FULL, upto, 31);
     };
-    long long total = 0, upto = 0;
-    int live = 0;
+    int total = 0, upto = 0, live = 0;
+    float size = 0.0f;                               // of the line, in numbers that cannot overflow
+#pragma unroll 1
     for (int b0 = 0; b0 < a.requests; b0 += 32 * EACH) {
         total += scan(b0, upto);
 #pragma unroll
-        for (int i = 0; i < EACH; ++i) live += __popc(__ballot_sync(FULL, lens[i] > 0));
+        for (int i = 0; i < EACH; ++i) {
+            live += __popc(__ballot_sync(FULL, lens[i] > 0));
+            size += (float)lens[i];
+        }
     }
-    const long long pairs = (long long)live * HV, tiles = total - pairs * PAIR_COST;
-    const int ctas = (int)min((long long)gridDim.x, max(1ll, max(pairs, tiles / MIN_TILES)));
+#pragma unroll
+    for (int off = 16; off > 0; off >>= 1) size += __shfl_xor_sync(FULL, size, off);
+    const bool too_long = (size / C::TW + (PAIR_COST + 2) * (float)live) * HV > 0.99f * LINE_PLACES;
+    const int pairs = live * HV, tiles = total - pairs * PAIR_COST;
+    const int ctas = min((int)gridDim.x, max(1, max(pairs, tiles / MIN_TILES)));
     const int cta = blockIdx.x;
-    // (a 64-bit division takes some hundred cycles; 32 bits hold the products of all but the longest lines)
-    const bool narrow = total <= 0xffffffffll / (ctas + 1);
-    auto share = [&](int c) { return narrow ? (long long)((unsigned)total * (unsigned)c / (unsigned)ctas) : total * c / ctas; };
-    auto owner = [&](long long place) {
-        return narrow ? (int)((((unsigned)place + 1u) * (unsigned)ctas - 1u) / (unsigned)total) : (int)(((place + 1) * ctas - 1) / total);
+    // equal shares, the first `rest` of them a place longer
+    const int each = total / ctas, rest = total - each * ctas;
+    auto share = [&](int c) { return c * each + min(c, rest); };
+    auto owner = [&](int place) {
+        const int longer = rest * (each + 1);
+        return place < longer ? place / (each + 1) : rest + (place - longer) / each;
     };
 
     // padded rows, and lengths that do not fit: zeros
+#pragma unroll 1
     for (int b = cta; b < a.requests; b += gridDim.x) {
-        if (valid_len(a, b) > 0) continue;
-        if (a.lens[b] != 0 && tid == 0) report_status(a.status, DEV_BAD_PAGE, 13);
+        const int len = a.lens[b];
+        if (valid_len(len, a.max_len) > 0 && !too_long) continue;
+        if (len != 0 && tid == 0) report_status(a.status, DEV_BAD_PAGE, 13);
+#pragma unroll 1
         for (int d = tid; d < H * HD / 4; d += THREADS) reinterpret_cast<float4*>(a.out)[(size_t)b * (H * HD / 4) + d] = make_float4(0.f, 0.f, 0.f, 0.f);
     }
-    if (cta >= ctas || total == 0) return;
-    const long long s0 = share(cta), s1 = share(cta + 1);
+    if (cta >= ctas || total == 0 || too_long) return;
+    const int s0 = share(cta), s1 = share(cta + 1);
 
     Cursor seg{};    // the first tile of this share
     {
-        long long base = 0;
+        int base = 0;
+#pragma unroll 1
         for (int b0 = 0; b0 < a.requests; b0 += 32 * EACH) {
-            const long long all = a.requests <= 32 * EACH ? total : scan(b0, upto);
+            const int all = a.requests <= 32 * EACH ? total : scan(b0, upto);
             if (s0 < base + all) {
                 const int at = __ffs(__ballot_sync(FULL, base + upto > s0)) - 1;      // the lane that holds the request
-                long long from = base + upto;
+                int from = base + upto, b = 0, len = 0, first = 0;
 #pragma unroll
                 for (int i = 0; i < EACH; ++i) from -= places(lens[i]);
-                int b = 0, len = 0;
-                long long first = 0;
 #pragma unroll
                 for (int i = 0; i < EACH; ++i) {
                     if (lens[i] > 0 && from <= s0) b = b0 + lane * EACH + i, len = lens[i], first = from;
@@ -872,18 +882,19 @@ __global__ void __launch_bounds__(THREADS, CTAS_PER_SM) paged_decode_kernel(Page
         }
     }
     seg.tiles = tiles_of<C>(seg.len);
-    seg.hv = narrow ? (int)((unsigned)(s0 - seg.at) / (unsigned)(seg.tiles + PAIR_COST)) : (int)((s0 - seg.at) / (seg.tiles + PAIR_COST));
-    seg.at += (long long)seg.hv * (seg.tiles + PAIR_COST);
-    seg.j = (int)max(0ll, s0 - seg.at - PAIR_COST);
+    seg.hv = (s0 - seg.at) / (seg.tiles + PAIR_COST);
+    seg.at += seg.hv * (seg.tiles + PAIR_COST);
+    seg.j = max(0, s0 - seg.at - PAIR_COST);
     if (seg.place() >= s1) return;                   // the share lies before the pair's first tile
 
+    auto seg_head = [&](const Cursor& c) { return divide(c.hv, a.by_tiles); };
     // Segment of the pair at the cursor, up to jend
     auto segment_of = [&](const Cursor& c, int& jend) {
-        jend = (int)min((long long)c.tiles, s1 - c.at - PAIR_COST);
+        jend = min(c.tiles, s1 - c.at - PAIR_COST);
         Segment s;
         s.b = c.b;
         s.len = c.len;
-        s.kv_h = c.hv / a.head_tiles;
+        s.kv_h = seg_head(c);
         const int ht = c.hv - s.kv_h * a.head_tiles;
         s.head0 = s.kv_h * G + ht * per;
         s.heads = min(per, G - ht * per);
@@ -891,8 +902,6 @@ __global__ void __launch_bounds__(THREADS, CTAS_PER_SM) paged_decode_kernel(Page
         s.stores = ht == 0;
         return s;
     };
-
-    auto seg_head = [&](const Cursor& c) { return c.hv / a.head_tiles; };
 
     // ---- this warp's copies: the share's tiles warp, warp + NW, ...; page numbers two tiles ahead ----
     Cursor ld = seg;
@@ -905,7 +914,7 @@ __global__ void __launch_bounds__(THREADS, CTAS_PER_SM) paged_decode_kernel(Page
         if (ahead.place() < s1) place1 = lookup_page<C>(a, ahead, lane);
     }
     int ld_head = seg_head(ld);
-    long long ld_place = ld.place();
+    int ld_place = ld.place();
     const unsigned char* kp = static_cast<const unsigned char*>(a.k_pages) + lane % C::CH * 16;
     const unsigned char* vp = static_cast<const unsigned char*>(a.v_pages) + lane % C::CH * 16;
     const uint32_t ring_at = smem_u32(ring);
@@ -927,10 +936,11 @@ __global__ void __launch_bounds__(THREADS, CTAS_PER_SM) paged_decode_kernel(Page
 
     int jend;
     Segment sg = segment_of(seg, jend);
-    Rows<C> rows;
-    rows.load(a, sg, warp, lane);
-#pragma unroll
+    request_rows<C>(a, sg, qs, xk, xv, warp, lane);
+    copy_commit();
+#pragma unroll 1
     for (int i = 0; i < STAGES - 1; ++i) fetch();
+    copy_wait<STAGES - 1>();          // the rows
 
     State<C> st;
     const float to2 = a.scale * LOG2E;
@@ -950,10 +960,13 @@ __global__ void __launch_bounds__(THREADS, CTAS_PER_SM) paged_decode_kernel(Page
         __syncthreads();
         return s_last != 0;
     };
+#pragma unroll 1
     while (true) {
-        rows.finish(a, sg, qs, xk, xv, warp, lane);
+        __syncwarp();
+        prepare_rows<C>(a, sg, qs, xk, xv, warp, lane);
         __syncthreads();
         st.start(qs, lane);
+#pragma unroll 1
         for (int j = seg.j + ((warp - done) & (NW - 1)); j < jend; j += NW) {     // this warp's tiles
             copy_wait<STAGES - 2>();
             __syncwarp();
@@ -972,22 +985,23 @@ __global__ void __launch_bounds__(THREADS, CTAS_PER_SM) paged_decode_kernel(Page
 
         const Segment cur = sg;
         const int j0 = seg.j, jn = jend, whole = seg.tiles;
-        const long long pair_at = seg.at;
-        const bool first = done == 0;
+        const int pair_at = seg.at;
         done += jn - j0;
         advance<C>(a, seg, jn - j0);
         const bool more = jn == whole && seg.place() < s1;
+        __syncthreads();
         if (more) {
             sg = segment_of(seg, jend);
-            rows.load(a, sg, warp, lane);            // arrive while the sums are joined
+            request_rows<C>(a, sg, qs, xk, xv, warp, lane);      // arrive while the sums are joined
+            copy_commit();
         }
-        __syncthreads();
 
         // ---- the four warps' sums, to the output or to the workspace ----
         const bool complete = j0 == 0 && jn == whole;
-        const size_t part = (size_t)cta * 2 + (first ? 0 : 1);
+        const size_t part = (size_t)cta * 2 + (j0 == 0 ? 1 : 0);
         float* out = a.out + ((size_t)cur.b * H + cur.head0) * HD;
         const int tasks = cur.heads * (HD / 4);      // four columns of a head
+#pragma unroll 1
         for (int e = tid; e < tasks; e += THREADS) {
             const int g = e / (HD / 4), d = (e - g * (HD / 4)) * 4;
             float top = -INFINITY, L = 0.0f;
@@ -1013,20 +1027,21 @@ __global__ void __launch_bounds__(THREADS, CTAS_PER_SM) paged_decode_kernel(Page
             }
         }
         if (!complete) {
-            Shared& p = pend[first ? 0 : 1];
+            Shared p;
             p.c0 = owner(pair_at + PAIR_COST);
             p.n = owner(pair_at + PAIR_COST + whole - 1) - p.c0 + 1;
-            p.shift = share(p.c0) < pair_at ? 1 : 0;
+            p.fan = Join<C>::fan_of(p.n, cur.heads);
             p.heads = cur.heads;
             p.out = out;
-            // The groups' counters: a group may begin with the CTA in which another pair's last group ends, and that one is
-            // not the first of its pair.
-            const int g0 = p.c0 + (cta - p.c0) / p.fan<C>() * p.fan<C>();
-            p.mine = last_of(p.n <= p.fan<C>() ? a.counters + p.c0 : a.counters + gridDim.x + 2 * g0 + (g0 == p.c0 ? 1 : 0),
-                             min(p.fan<C>(), p.c0 + p.n - g0));
+            // The groups' counters: a group may begin with the CTA in which another pair begins.
+            const int g0 = p.c0 + (cta - p.c0) / p.fan * p.fan;
+            p.mine = last_of(p.n <= p.fan ? a.counters + p.c0 : a.counters + gridDim.x + 2 * g0 + (g0 == p.c0 ? 1 : 0),
+                             min(p.fan, p.c0 + p.n - g0));
+            pend[j0 == 0 ? 1 : 0] = p;
         }
         if (!more) break;
-        __syncthreads();      // parked sums, q rows and new rows have been read
+        copy_wait<0>();
+        __syncthreads();      // the parked sums have been read
     }
     copy_wait<0>();
     __syncthreads();
@@ -1034,21 +1049,28 @@ __global__ void __launch_bounds__(THREADS, CTAS_PER_SM) paged_decode_kernel(Page
     // ---- the pairs whose last part was this CTA's; the rings are free now ----
 #pragma unroll 1
     for (int i = 0; i < 2; ++i) {
-        const Shared& p = pend[i];
+        const Shared p = pend[i];
         if (!p.mine) continue;
+        __syncthreads();
         Join<C> join;
-        const int fan = p.fan<C>();
-        if (p.n > fan) {
-            const int g0 = p.c0 + (cta - p.c0) / fan * fan;
-            join.run(a, p, g0, 1, min(fan, p.c0 + p.n - g0), pd_smem, tid);
-            join.store(a, p, g0, pd_smem, tid);
-            const int groups = (p.n + fan - 1) / fan;
-            if (!last_of(a.counters + p.c0, groups)) continue;
-            join.run(a, p, p.c0, fan, groups, pd_smem, tid);
-        } else {
-            join.run(a, p, p.c0, 1, p.n, pd_smem, tid);
+        float2* ml = reinterpret_cast<float2*>(a.part_ml);
+        const int g0 = p.c0 + (cta - p.c0) / p.fan * p.fan;
+        int at = 2 * g0, step = 2, n = min(p.fan, p.c0 + p.n - g0), odd = g0 == p.c0 ? 1 : 0;
+        bool last = true;
+#pragma unroll 1
+        while (true) {
+            join.run(a.part_o, ml, at, step, n, odd, p.heads, pd_smem, tid);
+            if (p.n <= p.fan || step == 1) break;
+            // the second table lies behind the parts; a pair's groups take the places of its first CTAs there
+            const int second = 2 * gridDim.x + p.c0;
+            n = (p.n + p.fan - 1) / p.fan;
+            join.store(a.part_o, ml, second + (g0 - p.c0) / p.fan, p.heads, pd_smem, tid);
+            last = last_of(a.counters + p.c0, n);
+            if (!last) break;
+            at = second, step = 1, odd = 0;
         }
-        join.finish(p, pd_smem, tid);
+        if (!last) continue;
+        join.finish(p.out, p.heads, pd_smem, tid);
     }
 }
 
@@ -1095,15 +1117,17 @@ PagedPlan paged_decode_plan(const HeadShape& hs, int kv_elem_bytes, int sm_count
     p.gt = kv_elem_bytes == 4 ? 8 : 4;
     while (p.gt < per) p.gt *= 2;
     p.ctas = sm_count * CTAS_PER_SM;
-    p.part_floats = (size_t)p.ctas * 2 * p.gt * (hs.head_dim + 2);
+    p.part_floats = (size_t)p.ctas * 3 * p.gt * (hs.head_dim + 2);
     return p;
 }
 
 cudaError_t launch_paged_decode(PagedDecodeArgs a, const PagedPlan& p, float* workspace, unsigned* counters, cudaStream_t s) {
+    a.max_len = (int)std::min<long long>((long long)a.table_width * a.page_rows, 0x7fffffff);
     a.by_page = fast_div(a.page_rows);
+    a.by_tiles = fast_div(p.head_tiles);
     a.head_tiles = p.head_tiles;
     a.part_o = workspace;
-    a.part_ml = workspace + (size_t)p.ctas * 2 * p.gt * a.hs.head_dim;
+    a.part_ml = workspace + (size_t)p.ctas * 3 * p.gt * a.hs.head_dim;
     a.counters = counters;
     const long long most = (long long)a.table_width * a.page_rows * a.hs.num_kv_heads * p.head_tiles;   // tiles, at one row each
     const int ctas = (int)std::min<long long>(p.ctas, std::max<long long>(1, std::min<long long>(most, 0x7fffffff) * a.requests));
