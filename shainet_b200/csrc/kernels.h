@@ -298,7 +298,7 @@ struct Q4GemvArgs {
     int M, N, K, group;
     int pass_rows;          // set by the launch: rows of one pass over the weights
 };
-cudaError_t launch_q4_gemv(Q4GemvArgs a, int sm_count, cudaStream_t s);
+cudaError_t launch_q4_gemv(const Q4GemvArgs& a, int sm_count, cudaStream_t s);
 
 // Sets the calling thread's message for shainet_attn_last_error().
 void set_last_error_message(const char* msg);

@@ -10,7 +10,7 @@
 // Arithmetic.  The weights are exact as bfloat16: a nibble is dropped into the mantissa of 128 and 136 subtracted (4
 // instructions for 4 values).  Activations are fp32 and enter as three bfloat16 planes each, x = hi + mid + lo exactly (24
 // bits cut into 8 + 8 + 8), so no operand is rounded.  m16n8k16 multiplications with fp32 accumulators; the sums of 32
-// inputs start from zero and are added in fp32 with their scale, so sums that the matrix units cut off stay short.
+// or 64 inputs start from zero and are added in fp32 with their scale, so sums that the matrix units cut off stay short.
 //   * One or two rows: the planes are the columns of one multiplication (2 rows x 3 planes of 8).
 //   * More rows: eight rows a multiplication, three of them for the planes, up to 40 rows a pass over the weights.
 //
@@ -98,7 +98,6 @@ __global__ void __launch_bounds__(256) q4_scales_kernel(const float* from, float
 }
 
 // ---- product ----
-__device__ __forceinline__ uint32_t smem_at(const void* p) { return static_cast<uint32_t>(__cvta_generic_to_shared(p)); }
 __device__ __forceinline__ void copy16(uint32_t dst, const void* src) {
     asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
 }
@@ -109,7 +108,7 @@ __device__ __forceinline__ void copy_wait() { asm volatile("cp.async.wait_group 
 // d += a b, or d = a b with FIRST
 template <bool FIRST>
 __device__ __forceinline__ void mma(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
-    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%10, %11, %12, %13};"
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%10, %11, %12, %13};"
                  : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
                  : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(FIRST ? 0.f : d[0]), "f"(FIRST ? 0.f : d[1]),
                    "f"(FIRST ? 0.f : d[2]), "f"(FIRST ? 0.f : d[3]));
@@ -136,50 +135,58 @@ __device__ __forceinline__ void planes(float x0, float x1, uint32_t (&p)[3]) {
     p[2] = __byte_perm(__float_as_uint(s0), __float_as_uint(s1), 0x7632);
 }
 
-// MT = 0: one or two rows, their planes kept in shared memory; else 8 * MT rows at most.
-template <int MT_, int NT_>
+// MT = 0: one or two rows, their planes kept in shared memory; else 8 * MT rows at most.  A ring place holds KU blocks of 64
+// inputs of each of NT blocks of outputs, and their scales.
+template <int MT_, int NT_, int G_>
 struct Cfg {
-    static constexpr int MT = MT_, NT = NT_;
+    static constexpr int MT = MT_, NT = NT_, G = G_;                  // G: inputs of a group
+    static constexpr int EVEN = G == 128 ? 2 : 1;                     // a warp's blocks of 64 inputs start with a group
+    static constexpr int KU = MT == 0 ? 4 : 1;
+    static constexpr int PLACE = KU * 640;                            // one block of outputs: 512 bytes a block of inputs, then scales
+    static constexpr int UNIT = NT * PLACE;
+    static constexpr int RING = MT == 0 ? 2 : NT == 1 ? 5 : 3;        // places of a warp's ring: one in use
+    static constexpr int AHEAD = MT <= 3 ? 2 : 1;                     // steps of x that are fetched ahead
     static constexpr int COLS = MT == 0 ? 8 : 8 * MT;                 // columns of the sums: planes and rows, or rows
-    static constexpr int UNIT = NT * 640;                             // a ring place: NT blocks, 128 bytes for the scales of each
-    static constexpr int RING = MT == 0 ? 8 : NT == 1 ? 6 : 4;        // places of a warp's ring
     static constexpr int RED = COLS + 2;                              // floats between outputs in the sums' meeting place
-    static constexpr int SUMS = (MT == 0 ? 2 : 1) * WARPS * NT * 16 * RED * 4;
+    static constexpr int SET = WARPS * NT * 16 * RED;                 // floats of a set's sums
+    static constexpr int SUMS = (MT == 0 ? 2 : 1) * SET * 4;
     static constexpr size_t FIXED = (size_t)WARPS * RING * UNIT + SUMS;
 };
 
-// Inputs that a warp owns: blocks [first, first + count) of 64.
-__host__ __device__ __forceinline__ int slice_of(int kbs) { return (kbs + WARPS - 1) / WARPS; }
-
 template <class C>
-__global__ void __launch_bounds__(THREADS, C::MT == 0 ? 2 : 1) q4_gemv_kernel(Q4GemvArgs a, int kbs, int stored, int blocks) {
-    constexpr int MT = C::MT, NT = C::NT;
+__global__ void __launch_bounds__(THREADS, C::MT == 0 ? (C::NT == 1 ? 3 : 2) : 1) q4_gemv_kernel(Q4GemvArgs a, int kbs, int stored, int blocks) {
+    constexpr int MT = C::MT, NT = C::NT, KU = C::KU, TM = MT == 0 ? 1 : MT;
     extern __shared__ __align__(16) unsigned char q4_smem[];
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
     unsigned char* ring = q4_smem + (size_t)warp * C::RING * C::UNIT;
     float* red = reinterpret_cast<float*>(q4_smem + (size_t)WARPS * C::RING * C::UNIT);
-    uint4* xs = reinterpret_cast<uint4*>(q4_smem + C::FIXED);          // MT = 0: [pairs of 16 inputs][32 lanes]
-    const int slice = slice_of(kbs), kb0 = min(warp * slice, kbs), kb1 = min(kb0 + slice, kbs), mine = kb1 - kb0;
+    unsigned char* xs = q4_smem + C::FIXED;                            // MT = 0: [pairs of 16 inputs][column][t][2 x 8 bytes]
+    const int slice = ((kbs + WARPS - 1) / WARPS + C::EVEN - 1) / C::EVEN * C::EVEN, kb0 = min(warp * slice, kbs), kb1 = min(kb0 + slice, kbs);
     const int sets = (blocks + NT - 1) / NT;                           // of NT blocks of 16 outputs
     const int m0 = blockIdx.y * a.pass_rows, rows = min(a.pass_rows, a.M - m0);
     const float* x = a.x + (size_t)m0 * a.K;
-    const int per_kb = a.group == 32 ? 2 : 1, kb_shift = a.group == 128 ? 1 : 0;
 
     // ---- copies: for every set of this CTA the blocks of the warp's slice ----
     int ld_set = blockIdx.x, ld_kb = kb0;
     uint32_t fill = 0;
-    const uint32_t ring_at = smem_at(ring);
+    const uint32_t ring_at = static_cast<uint32_t>(__cvta_generic_to_shared(ring)) + lane * 16;
     auto fetch = [&]() {
-        if (mine > 0 && ld_set < sets) {
+        if (kb0 < kb1 && ld_set < sets) {
+            const int cnt = min(KU, kb1 - ld_kb);
 #pragma unroll
             for (int i = 0; i < NT; ++i) {
                 const int nt = min(ld_set * NT + i, blocks - 1);       // behind the last block: read again, not used
-                copy16(ring_at + fill + i * 640 + lane * 16, a.q + ((size_t)nt * kbs + ld_kb) * 32 + lane);
-                if (lane < 4 * per_kb)
-                    copy16(ring_at + fill + i * 640 + 512 + lane * 16, a.scales + ((size_t)nt * stored + (ld_kb * per_kb >> kb_shift)) * 16 + lane * 4);
+                const uint32_t to = ring_at + fill + i * C::PLACE;
+                const uint4* q = a.q + ((size_t)nt * kbs + ld_kb) * 32 + lane;
+#pragma unroll
+                for (int u = 0; u < KU; ++u)
+                    if (u < cnt) copy16(to + u * 512, q + u * 32);
+                const int g0 = C::G == 32 ? 2 * ld_kb : C::G == 64 ? ld_kb : ld_kb >> 1, gn = C::G == 32 ? 2 * cnt : C::G == 64 ? cnt : (cnt + 1) >> 1;
+                if (lane < 4 * gn) copy16(to + KU * 512, a.scales + ((size_t)nt * stored + g0) * 16 + lane * 4);
             }
             fill = fill == (C::RING - 1) * C::UNIT ? 0 : fill + C::UNIT;
-            if (++ld_kb == kb1) ld_kb = kb0, ld_set += gridDim.x;
+            ld_kb += cnt;
+            if (ld_kb == kb1) ld_kb = kb0, ld_set += gridDim.x;
         }
         copy_commit();
     };
@@ -188,118 +195,170 @@ __global__ void __launch_bounds__(THREADS, C::MT == 0 ? 2 : 1) q4_gemv_kernel(Q4
     asm volatile("griddepcontrol.wait;" ::: "memory");                 // x may come from the kernel ahead, y may be read by it
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
 
-    // x of one row and input; zero behind the last input
-    auto x_at = [&](const float* row, int k) { return k < a.K ? __ldcg(row + k) : 0.0f; };
+    const bool even = (a.K & 1) == 0;
+    // inputs k and k + 1 of a row; zeros behind the last input
+    auto pair_at = [&](const float* row, int k, bool whole) {
+        if (whole) return __ldcg(reinterpret_cast<const float2*>(row + k));
+        return make_float2(k < a.K ? __ldcg(row + k) : 0.0f, k + 1 < a.K ? __ldcg(row + k + 1) : 0.0f);
+    };
     if constexpr (MT == 0) {
-        // column g: plane g / 2 of row g % 2
-        const int plane = g >> 1;
-        const bool on = plane < 3 && (g & 1) < rows;
-        const float* row = x + (size_t)((g & 1) < rows ? g & 1 : 0) * a.K;
+        // Column plane * rows + row of a multiplication; the other columns' sums are not looked at, they take the last one's.
+        // A lane makes the three planes of four inputs: eight steps of 16 inputs at a time, or four of both rows.
+        const int per = rows == 1 ? 8 : 4, m = rows == 1 ? 0 : g & 1, first = rows == 1 ? g : g >> 1;
+        const float* row = x + (size_t)m * a.K;
 #pragma unroll 2
-        for (int p = kb0 * 2; p < kb1 * 2; ++p) {
-            uint32_t b[4];
+        for (int s = kb0 * 4 + first; s < kb1 * 4; s += per) {
+            const int k = s * 16 + 2 * t;
+            const bool whole = even && s * 16 + 16 <= a.K;
+            const float2 v0 = pair_at(row, k, whole), v1 = pair_at(row, k + 8, whole);
+            uint32_t p0[3], p1[3];
+            planes(v0.x, v0.y, p0);
+            planes(v1.x, v1.y, p1);
 #pragma unroll
-            for (int h = 0; h < 4; ++h) {
-                const int k = p * 32 + (h >> 1) * 16 + (h & 1) * 8 + 2 * t;
-                uint32_t v[3];
-                planes(x_at(row, k), x_at(row, k + 1), v);
-                b[h] = !on ? 0u : plane == 0 ? v[0] : plane == 1 ? v[1] : v[2];
-            }
-            xs[(size_t)p * 32 + lane] = make_uint4(b[0], b[1], b[2], b[3]);
+            for (int p = 0; p < 3; ++p)
+                *reinterpret_cast<uint2*>(xs + ((size_t)(s >> 1) * 3 * rows + p * rows + m) * 64 + t * 16 + (s & 1) * 8) = make_uint2(p0[p], p1[p]);
         }
         __syncwarp();
     }
-    const float* xrow[MT == 0 ? 1 : MT];
-    if constexpr (MT > 0)
+
+    // More rows: x is fetched AHEAD steps (of eight rows and 32 inputs) ahead, straight from L2
+    constexpr int AHEAD = C::AHEAD, VN = AHEAD + 1;
+    const float* xrow[TM];
 #pragma unroll
-        for (int mt = 0; mt < MT; ++mt) xrow[mt] = x + (size_t)min(mt * 8 + g, rows - 1) * a.K;      // rows behind the last: not stored
-    const bool even = (a.K & 1) == 0;
+    for (int mt = 0; mt < TM; ++mt) xrow[mt] = x + (size_t)min(mt * 8 + g, rows - 1) * a.K + 2 * t;      // rows behind the last: not stored
+    float2 v[VN][4];
+    auto load_step = [&](float2(&to)[4], int kb, int step) {
+        const int h = step / TM, mt = step - h * TM, k = kb * 64 + h * 32;
+        const bool whole = even && kb * 64 + 64 <= a.K;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            if (whole) to[i] = __ldcg(reinterpret_cast<const float2*>(xrow[mt] + k + i * 8));
+            else {
+                const int at = k + i * 8 + 2 * t;
+                to[i] = make_float2(at < a.K ? __ldcg(xrow[mt] + k + i * 8) : 0.0f, at + 1 < a.K ? __ldcg(xrow[mt] + k + i * 8 + 1) : 0.0f);
+            }
+        }
+    };
+    if constexpr (MT > 0)
+        if (kb0 < kb1) {
+            load_step(v[0], kb0, 0);
+            if constexpr (AHEAD == 2) load_step(v[1], kb0, 1);
+        }
 
     uint32_t take = 0;
     int turn = 0;
 #pragma unroll 1
     for (int set = blockIdx.x; set < sets; set += gridDim.x, ++turn) {
-        float total[NT][MT == 0 ? 1 : MT][4];
+        float total[NT][TM][4];
 #pragma unroll
         for (int i = 0; i < NT; ++i)
 #pragma unroll
-            for (int mt = 0; mt < (MT == 0 ? 1 : MT); ++mt)
+            for (int mt = 0; mt < TM; ++mt)
 #pragma unroll
                 for (int c = 0; c < 4; ++c) total[i][mt][c] = 0.0f;
 #pragma unroll 1
-        for (int kb = kb0; kb < kb1; ++kb) {
+        for (int kb = kb0; kb < kb1; kb += KU) {
             copy_wait<C::RING - 2>();
             __syncwarp();
+            fetch();                                                   // into the place that the last turn was done with
             const unsigned char* unit = ring + take;
+            if constexpr (MT == 0) {
+                const int pair = 3 * rows * 64;
+                const unsigned char* xb = xs + (size_t)kb * 2 * pair + min(g, 3 * rows - 1) * 64 + t * 16;
+                const unsigned char* qb = unit + lane * 16;
+                const unsigned char* sb = unit + KU * 512 + g * 8;
+                const int cnt = kb1 - kb;
+                float c[NT][4];
+                auto add = [&](int i, const float(&d)[4], int at) {
+                    const float2 sc = *reinterpret_cast<const float2*>(sb + i * C::PLACE + at * 64);
+                    total[i][0][0] = fmaf(sc.x, d[0], total[i][0][0]);
+                    total[i][0][1] = fmaf(sc.x, d[1], total[i][0][1]);
+                    total[i][0][2] = fmaf(sc.y, d[2], total[i][0][2]);
+                    total[i][0][3] = fmaf(sc.y, d[3], total[i][0][3]);
+                };
 #pragma unroll
-            for (int h = 0; h < 2; ++h) {                              // 32 inputs
-                uint32_t w[NT][2];
-                float2 sc[NT];
+                for (int u = 0; u < KU; ++u) {
+                    if (u >= cnt) break;
+                    const uint4 b0 = *reinterpret_cast<const uint4*>(xb), b1 = *reinterpret_cast<const uint4*>(xb + pair);
+                    xb += 2 * pair;
 #pragma unroll
-                for (int i = 0; i < NT; ++i) {
-                    const uint2 v = *reinterpret_cast<const uint2*>(unit + i * 640 + lane * 16 + h * 8);
-                    w[i][0] = v.x, w[i][1] = v.y;
-                    sc[i] = *reinterpret_cast<const float2*>(unit + i * 640 + 512 + (per_kb == 2 ? h * 64 : 0) + g * 8);
+                    for (int i = 0; i < NT; ++i) {
+                        const uint4 w = *reinterpret_cast<const uint4*>(qb + i * C::PLACE + u * 512);
+                        uint32_t op[4][4];
+                        unpack(w.x, op[0]), unpack(w.y, op[1]), unpack(w.z, op[2]), unpack(w.w, op[3]);
+                        if (C::G == 128 && (u & 1)) mma<false>(c[i], op[0], b0.x, b0.y);
+                        else mma<true>(c[i], op[0], b0.x, b0.y);
+                        mma<false>(c[i], op[1], b0.z, b0.w);
+                        if constexpr (C::G == 32) {
+                            float d[4];
+                            mma<true>(d, op[2], b1.x, b1.y);
+                            mma<false>(d, op[3], b1.z, b1.w);
+                            add(i, c[i], 2 * u);
+                            add(i, d, 2 * u + 1);
+                        } else {
+                            mma<false>(c[i], op[2], b1.x, b1.y);
+                            mma<false>(c[i], op[3], b1.z, b1.w);
+                            if (C::G == 64) add(i, c[i], u);
+                            else if ((u & 1) || u + 1 == cnt) add(i, c[i], u >> 1);
+                        }
+                    }
                 }
+            } else {
                 uint32_t op[NT][2][4];
+                float2 sc[NT];
+                const int next = kb + 1 < kb1 ? kb + 1 : kb0;
 #pragma unroll
-                for (int i = 0; i < NT; ++i) unpack(w[i][0], op[i][0]), unpack(w[i][1], op[i][1]);
-                if constexpr (MT == 0) {
-                    const uint4 b = xs[(size_t)(kb * 2 + h) * 32 + lane];
+                for (int s = 0; s < 2 * MT; ++s) {
+                    const int h = s / MT, mt = s - h * MT;
+                    if (s + AHEAD < 2 * MT) load_step(v[(s + AHEAD) % VN], kb, s + AHEAD);
+                    else load_step(v[(s + AHEAD) % VN], next, s + AHEAD - 2 * MT);
+                    if (mt == 0) {
+#pragma unroll
+                        for (int i = 0; i < NT; ++i) {
+                            const uint2 w = *reinterpret_cast<const uint2*>(unit + i * C::PLACE + lane * 16 + h * 8);
+                            unpack(w.x, op[i][0]), unpack(w.y, op[i][1]);
+                            sc[i] = *reinterpret_cast<const float2*>(unit + i * C::PLACE + 512 + (C::G == 32 ? h * 64 : 0) + g * 8);
+                        }
+                    }
+                    uint32_t b[4][3];
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) planes(v[s % VN][i].x, v[s % VN][i].y, b[i]);
 #pragma unroll
                     for (int i = 0; i < NT; ++i) {
                         float c[4];
-                        mma<true>(c, op[i][0], b.x, b.y);
-                        mma<false>(c, op[i][1], b.z, b.w);
-                        total[i][0][0] = fmaf(sc[i].x, c[0], total[i][0][0]);
-                        total[i][0][1] = fmaf(sc[i].x, c[1], total[i][0][1]);
-                        total[i][0][2] = fmaf(sc[i].y, c[2], total[i][0][2]);
-                        total[i][0][3] = fmaf(sc[i].y, c[3], total[i][0][3]);
+                        mma<true>(c, op[i][0], b[0][2], b[1][2]);
+                        mma<false>(c, op[i][1], b[2][2], b[3][2]);
+                        mma<false>(c, op[i][0], b[0][1], b[1][1]);
+                        mma<false>(c, op[i][1], b[2][1], b[3][1]);
+                        mma<false>(c, op[i][0], b[0][0], b[1][0]);
+                        mma<false>(c, op[i][1], b[2][0], b[3][0]);
+                        total[i][mt][0] = fmaf(sc[i].x, c[0], total[i][mt][0]);
+                        total[i][mt][1] = fmaf(sc[i].x, c[1], total[i][mt][1]);
+                        total[i][mt][2] = fmaf(sc[i].y, c[2], total[i][mt][2]);
+                        total[i][mt][3] = fmaf(sc[i].y, c[3], total[i][mt][3]);
                     }
-                } else {
-                    const int k0 = kb * 64 + h * 32 + 2 * t;
-                    const bool whole = even && kb * 64 + 64 <= a.K;
+                }
+                // what is under way for the next block stands where that one looks for it
+                constexpr int R = 2 * MT % VN;
+                if constexpr (R != 0) {
+                    static_assert(AHEAD == 2, "two of three places to move");
 #pragma unroll
-                    for (int mt = 0; mt < MT; ++mt) {
-                        float2 v[4];
-                        if (whole) {
-#pragma unroll
-                            for (int i = 0; i < 4; ++i) v[i] = __ldcg(reinterpret_cast<const float2*>(xrow[mt] + k0 + i * 8));
-                        } else {
-#pragma unroll
-                            for (int i = 0; i < 4; ++i) v[i] = make_float2(x_at(xrow[mt], k0 + i * 8), x_at(xrow[mt], k0 + i * 8 + 1));
-                        }
-                        uint32_t b[4][3];
-#pragma unroll
-                        for (int i = 0; i < 4; ++i) planes(v[i].x, v[i].y, b[i]);
-#pragma unroll
-                        for (int i = 0; i < NT; ++i) {
-                            float c[4];
-                            mma<true>(c, op[i][0], b[0][2], b[1][2]);
-                            mma<false>(c, op[i][1], b[2][2], b[3][2]);
-                            mma<false>(c, op[i][0], b[0][1], b[1][1]);
-                            mma<false>(c, op[i][1], b[2][1], b[3][1]);
-                            mma<false>(c, op[i][0], b[0][0], b[1][0]);
-                            mma<false>(c, op[i][1], b[2][0], b[3][0]);
-                            total[i][mt][0] = fmaf(sc[i].x, c[0], total[i][mt][0]);
-                            total[i][mt][1] = fmaf(sc[i].x, c[1], total[i][mt][1]);
-                            total[i][mt][2] = fmaf(sc[i].y, c[2], total[i][mt][2]);
-                            total[i][mt][3] = fmaf(sc[i].y, c[3], total[i][mt][3]);
-                        }
+                    for (int i = 0; i < 4; ++i) {
+                        const float2 w0 = v[R][i], w1 = v[(R + 1) % VN][i];
+                        v[0][i] = w0, v[1][i] = w1;
                     }
                 }
             }
             __syncwarp();
             take = take == (C::RING - 1) * C::UNIT ? 0 : take + C::UNIT;
-            fetch();
         }
         // ---- the warps' sums ----
-        float* meet = red + (MT == 0 ? (turn & 1) * (WARPS * 16 * C::RED) : 0);
+        float* meet = red + (MT == 0 ? (turn & 1) * C::SET : 0);
         float* to = meet + warp * NT * 16 * C::RED;
 #pragma unroll
         for (int i = 0; i < NT; ++i)
 #pragma unroll
-            for (int mt = 0; mt < (MT == 0 ? 1 : MT); ++mt)
+            for (int mt = 0; mt < TM; ++mt)
 #pragma unroll
                 for (int r = 0; r < 2; ++r)
                     *reinterpret_cast<float2*>(to + (i * 16 + g + 8 * r) * C::RED + mt * 8 + 2 * t) = make_float2(total[i][mt][2 * r], total[i][mt][2 * r + 1]);
@@ -307,15 +366,16 @@ __global__ void __launch_bounds__(THREADS, C::MT == 0 ? 2 : 1) q4_gemv_kernel(Q4
         if constexpr (MT == 0) {
             // one warp adds, another one every time; the next sums go to the other half
             if (warp == (turn & (WARPS - 1))) {
-                const int n = lane & 15, m = lane >> 4, out = set * 16 + n;
-                if (m < rows && out < a.N) {
+#pragma unroll 1
+                for (int e = lane; e < NT * 16 * rows; e += 32) {
+                    const int m = e / (NT * 16), n = e - m * (NT * 16), out = set * (NT * 16) + n;
                     float sum = 0.0f;
 #pragma unroll
                     for (int w = 0; w < WARPS; ++w) {
-                        const float* s = meet + (w * 16 + n) * C::RED + m;
-                        sum += s[4] + s[2] + s[0];
+                        const float* s = meet + (w * (NT * 16) + n) * C::RED + m;
+                        sum += s[2 * rows] + s[rows] + s[0];
                     }
-                    a.y[(size_t)(m0 + m) * a.N + out] = sum;
+                    if (out < a.N) a.y[(size_t)(m0 + m) * a.N + out] = sum;
                 }
             }
         } else {
@@ -333,11 +393,13 @@ __global__ void __launch_bounds__(THREADS, C::MT == 0 ? 2 : 1) q4_gemv_kernel(Q4
     copy_wait<0>();
 }
 
-template <int MT, int NT>
+size_t plane_bytes(const Q4GemvArgs& a) { return (size_t)blocks_of(a.K, 64) * 2 * 3 * a.M * 64; }
+
+template <int MT, int NT, int G>
 cudaError_t launch(const Q4GemvArgs& a, int sm_count, cudaStream_t s) {
-    using C = Cfg<MT, NT>;
+    using C = Cfg<MT, NT, G>;
     const int kbs = blocks_of(a.K, 64), blocks = blocks_of(a.N, 16), sets = blocks_of(blocks, NT);
-    const size_t smem = C::FIXED + (MT == 0 ? (size_t)kbs * 1024 : 0);
+    const size_t smem = C::FIXED + (MT == 0 ? plane_bytes(a) : 0);
     static std::atomic<unsigned long long> configured{0};   // bit per device
     int dev = 0;
     cudaError_t e = cudaGetDevice(&dev);
@@ -348,7 +410,7 @@ cudaError_t launch(const Q4GemvArgs& a, int sm_count, cudaStream_t s) {
         if (dev < 64) configured.fetch_or(1ull << dev, std::memory_order_release);
     }
     const int passes = blocks_of(a.M, a.pass_rows);
-    const int per_sm = MT == 0 && smem <= 112 * 1024 ? 2 : 1;
+    const int per_sm = MT == 0 ? std::max(1, std::min(NT == 1 ? 3 : 2, (int)(227 * 1024 / (smem + 1024)))) : 1;
     cudaLaunchConfig_t cfg{};
     cfg.gridDim = dim3(std::min(sets, std::max(1, sm_count * per_sm / std::min(passes, per_sm))), passes);
     cfg.blockDim = dim3(THREADS);
@@ -362,28 +424,37 @@ cudaError_t launch(const Q4GemvArgs& a, int sm_count, cudaStream_t s) {
     return cudaLaunchKernelEx(&cfg, q4_gemv_kernel<C>, a, kbs, stored_groups(a.K, a.group), blocks);
 }
 
-template <int MT>
+template <int MT, int G>
 cudaError_t launch_rows(const Q4GemvArgs& a, int sm_count, cudaStream_t s) {
-    // four blocks of outputs share the planes of x where that still leaves a CTA for most SMs
-    return blocks_of(a.N, 16) >= 4 * (sm_count * 3 / 4) ? launch<MT, 4>(a, sm_count, s) : launch<MT, 1>(a, sm_count, s);
+    // blocks of outputs that share the planes of x: four or two where that still leaves a CTA for most SMs (4096 x 4096, 16
+    // rows: 24 us with one, 15 us with two; 8200 x 2048, 33 rows: 31 us with two, 21 us with four)
+    const long long work = (long long)blocks_of(a.N, 16) * blocks_of(a.M, a.pass_rows), most = sm_count * 3 / 4;
+    return work >= 4 * most ? launch<MT, 4, G>(a, sm_count, s) : work >= 2 * most ? launch<MT, 2, G>(a, sm_count, s) : launch<MT, 1, G>(a, sm_count, s);
+}
+
+template <int G>
+cudaError_t launch_group(Q4GemvArgs a, int sm_count, cudaStream_t s) {
+    a.pass_rows = a.M;
+    if (a.M <= 2 && Cfg<0, 1, G>::FIXED + plane_bytes(a) <= SMEM_MAX) {
+        // two blocks of outputs share the reads of x's planes where every CTA has several of them
+        return blocks_of(a.N, 16) >= 8 * sm_count && Cfg<0, 2, G>::FIXED + plane_bytes(a) <= 112 * 1024 ? launch<0, 2, G>(a, sm_count, s) : launch<0, 1, G>(a, sm_count, s);
+    }
+    a.pass_rows = blocks_of(a.M, blocks_of(a.M, 8 * MAX_MT));
+    switch (blocks_of(a.pass_rows, 8)) {
+        case 1: return launch_rows<1, G>(a, sm_count, s);
+        case 2: return launch_rows<2, G>(a, sm_count, s);
+        case 3: return launch_rows<3, G>(a, sm_count, s);
+        case 4: return launch_rows<4, G>(a, sm_count, s);
+        default: return launch_rows<5, G>(a, sm_count, s);
+    }
 }
 
 }  // namespace
 
 namespace shainet {
 
-cudaError_t launch_q4_gemv(Q4GemvArgs a, int sm_count, cudaStream_t s) {
-    a.pass_rows = a.M;
-    if (a.M <= 2 && Cfg<0, 1>::FIXED + (size_t)blocks_of(a.K, 64) * 1024 <= SMEM_MAX) return launch<0, 1>(a, sm_count, s);
-    const int passes = blocks_of(a.M, 8 * MAX_MT);
-    a.pass_rows = blocks_of(a.M, passes);
-    switch (blocks_of(a.pass_rows, 8)) {
-        case 1: return launch_rows<1>(a, sm_count, s);
-        case 2: return launch_rows<2>(a, sm_count, s);
-        case 3: return launch_rows<3>(a, sm_count, s);
-        case 4: return launch_rows<4>(a, sm_count, s);
-        default: return launch_rows<5>(a, sm_count, s);
-    }
+cudaError_t launch_q4_gemv(const Q4GemvArgs& a, int sm_count, cudaStream_t s) {
+    return a.group == 32 ? launch_group<32>(a, sm_count, s) : a.group == 64 ? launch_group<64>(a, sm_count, s) : launch_group<128>(a, sm_count, s);
 }
 
 }  // namespace shainet
