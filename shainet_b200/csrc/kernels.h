@@ -232,8 +232,11 @@ struct PagedPlanArgs {
     int* slots;             // [max_tokens]
     int* status;            // [2]
     int requests, table_width, page_rows, num_pages, max_tokens;
+    // set by the launch
+    int max_len;            // positions a table row holds
+    FastDiv by_page;        // division by page_rows
 };
-cudaError_t launch_paged_plan(const PagedPlanArgs& a, cudaStream_t s);
+cudaError_t launch_paged_plan(PagedPlanArgs a, cudaStream_t s);
 
 // One decode token for each of `requests` requests over pages: see shainet_attn_paged_decode_dev.
 struct PagedDecodeArgs {

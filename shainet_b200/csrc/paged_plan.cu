@@ -12,15 +12,16 @@
 // that every CTA does for itself in shared memory, one or two dependent loads per output.  Large steps are spread over
 // one cluster of eight CTAs, whose barrier separates the reads of lens and free_count from the writes of lens_out and
 // free_count_out, which may be the same arrays; small ones take one CTA.
+#include <algorithm>
+#include <atomic>
+#include "../../include/shainet_attn.h"
 #include "kernels.h"
-#include "paged_index.h"
 
 namespace shainet {
 
 namespace {
 
-constexpr int PLAN_THREADS = 1024;
-constexpr int PLAN_WARPS = PLAN_THREADS / 32;
+constexpr int PLAN_THREADS = 1024;      // at most; a small step takes 256
 constexpr int PLAN_CLUSTER = 8;
 constexpr unsigned FULL = 0xffffffffu;
 enum PlanStatus { PLAN_OK = 0, PLAN_SHORT = 1, PLAN_LENGTH = 2, PLAN_TOKENS = 3, PLAN_STACK = 4 };
@@ -32,8 +33,17 @@ struct Sums {
 
 __device__ __forceinline__ Sums operator+(Sums a, Sums b) { return {a.tokens + b.tokens, a.grow + b.grow, a.shrink + b.shrink}; }
 
-__device__ __forceinline__ Sums shfl_up(Sums v, int off) {
-    return {__shfl_up_sync(FULL, v.tokens, off), __shfl_up_sync(FULL, v.grow, off), __shfl_up_sync(FULL, v.shrink, off)};
+// Sums over the lanes up to this one.
+__device__ __forceinline__ Sums scan_warp(Sums v, int lane) {
+#pragma unroll
+    for (int off = 1; off < 32; off <<= 1) {
+        const Sums up{__shfl_up_sync(FULL, v.tokens, off), __shfl_up_sync(FULL, v.grow, off), __shfl_up_sync(FULL, v.shrink, off)};
+        if (lane >= off) v = v + up;
+    }
+    return v;
+}
+__device__ __forceinline__ Sums of_lane(Sums v, int from) {
+    return {__shfl_sync(FULL, v.tokens, from), __shfl_sync(FULL, v.grow, from), __shfl_sync(FULL, v.shrink, from)};
 }
 
 // The last r with sums[r] <= x (sums is non-decreasing, sums[0] == 0): the request that owns element x.
@@ -47,62 +57,66 @@ __device__ __forceinline__ int owner_of(const int* sums, int n, int x) {
     return lo;
 }
 
-__device__ __forceinline__ Sums change_of(int len, int delta, int page_rows) {
-    const int before = pages_for(len, page_rows), after = pages_for((long long)len + delta, page_rows);
+// n / P rounded up
+__device__ __forceinline__ int pages_of(int n, FastDiv by, int page_rows) {
+    const int q = divide(n, by);
+    return q + (n > q * page_rows ? 1 : 0);
+}
+
+__device__ __forceinline__ Sums change_of(int len, int delta, FastDiv by, int page_rows) {
+    const int before = pages_of(len, by, page_rows), after = pages_of(len + delta, by, page_rows);
     return {delta > 0 ? delta : 0, after > before ? after - before : 0, before > after ? before - after : 0};
 }
 
 __global__ void __launch_bounds__(PLAN_THREADS) paged_plan_kernel(PagedPlanArgs a) {
     extern __shared__ int plan_smem[];
-    const int R = a.requests, P = a.page_rows;
+    const int R = a.requests, P = a.page_rows, T = blockDim.x, W = T / 32;
     int* s_len = plan_smem;
     int* s_delta = s_len + R;
     int* s_new = s_delta + R;     // exclusive sums over the requests
     int* s_grow = s_new + R;
     int* s_shrink = s_grow + R;
-    __shared__ Sums warp_sums[PLAN_WARPS];
+    __shared__ Sums warp_sums[32];
     __shared__ int s_bad;
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     if (tid == 0) s_bad = R;
+    // the arrays may come from the kernel ahead in the stream; the next one may launch and wait for this one's end
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     const int f = a.free_count[0];
     __syncthreads();
-    for (int r = tid; r < R; r += PLAN_THREADS) {
-        const int len = a.lens[r];
-        int delta = a.delta[r];
+    // a length or step that does not fit becomes an empty request and ends in an error below
+    for (int r = tid; r < R; r += T) {
+        int len = a.lens[r], delta = a.delta[r];
         const long long after = (long long)len + delta;
-        if (!length_fits(len, a.table_width, P) || after < 0 || after > (long long)a.table_width * P) {
+        if ((unsigned)len > (unsigned)a.max_len || after < 0 || after > a.max_len) {
             atomicMin(&s_bad, r);
             delta = 0;
         }
         s_len[r] = len;
         s_delta[r] = delta;
     }
-    __syncthreads();
-    // a thread sums a run of requests, the runs are scanned over the CTA; a length that does not fit has change 0 and
-    // ends in an error below, its page count is not used
-    const int run = (R + PLAN_THREADS - 1) / PLAN_THREADS;
-    const int r0 = min(tid * run, R), r1 = min(r0 + run, R);
+    // a thread sums a run of requests, the runs are scanned over the CTA
+    const int run = (R + T - 1) / T, r0 = min(tid * run, R), r1 = min(r0 + run, R);
+    if (run > 1) __syncthreads();
+    auto change = [&](int r) {
+        const int len = s_len[r];
+        return (unsigned)len > (unsigned)a.max_len ? Sums{0, 0, 0} : change_of(len, s_delta[r], a.by_page, P);
+    };
     Sums mine{0, 0, 0};
-    for (int r = r0; r < r1; ++r) mine = mine + change_of(s_len[r], s_delta[r], P);
-    Sums incl = mine;
-#pragma unroll
-    for (int off = 1; off < 32; off <<= 1) {
-        const Sums up = shfl_up(incl, off);
-        if (lane >= off) incl = incl + up;
-    }
+    for (int r = r0; r < r1; ++r) mine = mine + change(r);
+    const Sums incl = scan_warp(mine, lane);
     if (lane == 31) warp_sums[warp] = incl;
     __syncthreads();
-    Sums base{0, 0, 0}, total{0, 0, 0};
-    for (int w = 0; w < PLAN_WARPS; ++w) {
-        if (w == warp) base = total;
-        total = total + warp_sums[w];
-    }
-    Sums at{base.tokens + incl.tokens - mine.tokens, base.grow + incl.grow - mine.grow, base.shrink + incl.shrink - mine.shrink};
+    const Sums warps = scan_warp(lane < W ? warp_sums[lane] : Sums{0, 0, 0}, lane);
+    const Sums total = of_lane(warps, 31), base = of_lane(warps, warp > 0 ? warp - 1 : 0);
+    Sums at{incl.tokens - mine.tokens, incl.grow - mine.grow, incl.shrink - mine.shrink};
+    if (warp > 0) at = at + base;
     for (int r = r0; r < r1; ++r) {
         s_new[r] = (int)at.tokens;     // exact where it is used: the total is at most max_tokens
         s_grow[r] = at.grow;
         s_shrink[r] = at.shrink;
-        at = at + change_of(s_len[r], s_delta[r], P);
+        at = at + change(r);
     }
     __syncthreads();
     const int freed = total.shrink;
@@ -120,7 +134,7 @@ __global__ void __launch_bounds__(PLAN_THREADS) paged_plan_kernel(PagedPlanArgs 
     if (ctas > 1)
         asm volatile("barrier.cluster.arrive.aligned;\n barrier.cluster.wait.aligned;" ::: "memory");
 
-    const int t0 = rank * PLAN_THREADS + tid, step = ctas * PLAN_THREADS;
+    const int t0 = rank * T + tid, step = ctas * T;
     const bool ok = code == PLAN_OK;
     if (t0 == 0) {
         a.status[0] = code;
@@ -139,7 +153,7 @@ __global__ void __launch_bounds__(PLAN_THREADS) paged_plan_kernel(PagedPlanArgs 
     // the k-th freed page
     auto freed_page = [&](int k) {
         const int r = owner_of(s_shrink, R, k);
-        return a.block_table[(size_t)r * a.table_width + pages_for((long long)s_len[r] + s_delta[r], P) + k - s_shrink[r]];
+        return a.block_table[(size_t)r * a.table_width + pages_of(s_len[r] + s_delta[r], a.by_page, P) + k - s_shrink[r]];
     };
     // the i-th page that is popped
     auto popped_page = [&](int i) {
@@ -149,16 +163,15 @@ __global__ void __launch_bounds__(PLAN_THREADS) paged_plan_kernel(PagedPlanArgs 
     for (int k = t0; k < freed; k += step) a.free_pages[f + k] = freed_page(k);
     for (int i = t0; i < total.grow; i += step) {
         const int r = owner_of(s_grow, R, i);
-        a.block_table[(size_t)r * a.table_width + pages_for(s_len[r], P) + i - s_grow[r]] = popped_page(i);
+        a.block_table[(size_t)r * a.table_width + pages_of(s_len[r], a.by_page, P) + i - s_grow[r]] = popped_page(i);
     }
     for (int t = t0; t < a.max_tokens; t += step) {
         int slot = -1;
         if (t < total.tokens) {
             const int r = owner_of(s_new, R, t);
-            const long long pos = (long long)s_len[r] + t - s_new[r];
-            const int col = (int)(pos / P), before = pages_for(s_len[r], P);
+            const int pos = s_len[r] + (t - s_new[r]), col = divide(pos, a.by_page), before = pages_of(s_len[r], a.by_page, P);
             const int page = col < before ? a.block_table[(size_t)r * a.table_width + col] : popped_page(s_grow[r] + col - before);
-            slot = (int)(page * (long long)P + pos % P);
+            slot = (int)((long long)page * P + (pos - col * P));
         }
         a.slots[t] = slot;
     }
@@ -166,25 +179,35 @@ __global__ void __launch_bounds__(PLAN_THREADS) paged_plan_kernel(PagedPlanArgs 
 
 }  // namespace
 
-cudaError_t launch_paged_plan(const PagedPlanArgs& a, cudaStream_t s) {
+cudaError_t launch_paged_plan(PagedPlanArgs a, cudaStream_t s) {
+    a.max_len = (int)std::min<long long>((long long)a.table_width * a.page_rows, 0x7fffffff);
+    a.by_page = fast_div(a.page_rows);
     // one CTA up to 8 tokens and 2 requests a thread: a cluster's launch and barrier cost more than it saves there
     const bool wide = a.max_tokens > 8 * PLAN_THREADS || a.requests > 2 * PLAN_THREADS;
+    const bool narrow = a.max_tokens <= 1024 && a.requests <= 256;
     const size_t smem = (size_t)a.requests * 5 * sizeof(int);
-    if (smem > 48 * 1024) {
-        cudaError_t e = cudaFuncSetAttribute(paged_plan_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+    static std::atomic<unsigned long long> configured{0};   // bit per device
+    int dev = 0;
+    cudaError_t e = cudaGetDevice(&dev);
+    if (e != cudaSuccess) return e;
+    if (dev >= 64 || !(configured.load(std::memory_order_acquire) >> dev & 1ull)) {
+        e = cudaFuncSetAttribute(paged_plan_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, SHAINET_ATTN_PAGED_MAX_REQUESTS * 5 * (int)sizeof(int));
         if (e != cudaSuccess) return e;
+        if (dev < 64) configured.fetch_or(1ull << dev, std::memory_order_release);
     }
     cudaLaunchConfig_t cfg{};
     cfg.gridDim = dim3(wide ? PLAN_CLUSTER : 1);
-    cfg.blockDim = dim3(PLAN_THREADS);
+    cfg.blockDim = dim3(narrow ? 256 : PLAN_THREADS);
     cfg.dynamicSmemBytes = smem;
     cfg.stream = s;
-    cudaLaunchAttribute at[1];
-    at[0].id = cudaLaunchAttributeClusterDimension;
-    at[0].val.clusterDim.x = cfg.gridDim.x;
-    at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
+    cudaLaunchAttribute at[2];
+    at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    at[0].val.programmaticStreamSerializationAllowed = 1;
+    at[1].id = cudaLaunchAttributeClusterDimension;
+    at[1].val.clusterDim.x = cfg.gridDim.x;
+    at[1].val.clusterDim.y = at[1].val.clusterDim.z = 1;
     cfg.attrs = at;
-    cfg.numAttrs = 1;
+    cfg.numAttrs = wide ? 2 : 1;
     return cudaLaunchKernelEx(&cfg, paged_plan_kernel, a);
 }
 
