@@ -289,8 +289,9 @@ struct PagedCopyArgs {
     const int* index;
     int num_pages, page_rows, num_kv_heads, capacity, row0, rows, row_bytes;
     AttnStatus* status;
+    FastDiv by_page;        // set by the launch: division by page_rows
 };
-cudaError_t launch_paged_copy(const PagedCopyArgs& a, bool scatter, cudaStream_t s);
+cudaError_t launch_paged_copy(PagedCopyArgs a, bool scatter, cudaStream_t s);
 
 // y[M, N] = x[M, K] . dequant(W) over 4-bit weights in the layout of q4_gemv.cu.
 struct Q4GemvArgs {
