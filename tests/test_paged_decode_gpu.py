@@ -214,36 +214,54 @@ def test_two_handles_on_two_streams_at_once(ctx):
 
 @pytest.mark.parametrize("kv", ["f32", "bf16"])
 def test_replayed_graph_follows_growing_requests(ctx, kv):
-    """One capture; lengths and tables change on the device between replays, from a single row to several splits."""
+    """One capture; lengths, tables and pages change on the device between replays, from nothing to several splits."""
     import torch
-    b = Batch(ctx, LAYOUTS["Q8B"], [1, 40, 0, 3000], 16, kv, 21)
+    b = Batch(ctx, LAYOUTS["g7"] | dict(bias=False), [1, 40, 0, 3000], 16, kv, 21)
     stream, graph = torch.cuda.Stream(), torch.cuda.CUDAGraph()
     with torch.cuda.graph(graph, stream=stream):
         b.call(stream=stream.cuda_stream)
-    small = Batch(ctx, LAYOUTS["Q8B"], [1, 1, 1, 1], 16, kv, 22)
-    for lens in ([1, 40, 0, 3000], [1, 33, 0, 5], [0, 0, 0, 0], [0, 40, 0, 2999]):
-        c = Batch(ctx, LAYOUTS["Q8B"], lens, 16, kv, 23 + sum(lens))
-        # the captured buffers take the other batch's contents where they fit: rows are compared with its own eager call
-        b.tl.copy_(c.tl)
-        b.tq.copy_(c.tq), b.tkn.copy_(c.tkn), b.tvn.copy_(c.tvn)
+    for lens in ([1, 33, 0, 5], [0, 0, 0, 0], [7, 40, 0, 2999], [1, 1, 1, 1]):
+        c = Batch(ctx, LAYOUTS["g7"] | dict(bias=False), lens, 16, kv, 23 + sum(lens))      # the same parameters, other contents
+        b.tk[:c.NP].copy_(c.tk), b.tv[:c.NP].copy_(c.tv)
+        want = c.check()
+        b.tl.copy_(c.tl), b.tq.copy_(c.tq), b.tkn.copy_(c.tkn), b.tvn.copy_(c.tvn)
         b.tt.fill_(2**31 - 1)
         b.tt[:, :c.W].copy_(c.tt)
-        b.tk[:c.NP].copy_(c.tk), b.tv[:c.NP].copy_(c.tv)
-        want = c.check() if not any(lens) or "q_norm" not in b.kw else None
         torch.cuda.synchronize()
         graph.replay()
         torch.cuda.synchronize()
         ctx.sync()
-        got = b.out.cpu().numpy()[:4]
-        if want is not None:
-            assert np.array_equal(got, want)
-        # the block's norm weights are the captured one's: compare with an eager call of the same object
-        b.out.fill_(float("nan"))
-        b.call()
-        ctx.sync()
-        assert np.array_equal(got, b.out.cpu().numpy()[:4])
+        assert np.array_equal(b.out.cpu().numpy()[:4], want)
+        assert torch.equal(b.tk[:c.NP].view(torch.uint8), c.tk.view(torch.uint8)) and torch.equal(b.tv[:c.NP].view(torch.uint8), c.tv.view(torch.uint8))
         c.close()
-    small.close()
+    b.close()
+
+
+@pytest.mark.parametrize("kv", ["f32", "bf16"])
+def test_pages_that_are_only_read_may_be_shared(ctx, kv):
+    """Three requests with one prefix: their tables name the same pages up to the one that each writes into."""
+    import torch
+    b = Batch(ctx, LAYOUTS["L1B"], [100, 75, 70], 16, kv, 61)
+    b.table[1, :4] = b.table[2, :4] = b.table[0, :4]
+    b.tt.copy_(torch.from_numpy(b.table))
+    torch.cuda.synchronize()
+    b.check()
+    b.close()
+
+
+@pytest.mark.parametrize("kv", ["f32", "bf16"])
+@pytest.mark.parametrize("scale", [0.0, -0.125], ids=["zero", "negative"])
+def test_other_scales(ctx, scale, kv):
+    b = Batch(ctx, LAYOUTS["L1B"], [1, 33, 500], 16, kv, 62)
+    b.scale = scale
+    b.check()
+    b.close()
+
+
+def test_a_thousand_short_requests(ctx):
+    rng = np.random.default_rng(63)
+    b = Batch(ctx, LAYOUTS["one"], rng.integers(0, 40, 1000), 8, "f32", 64)
+    b.check()
     b.close()
 
 
