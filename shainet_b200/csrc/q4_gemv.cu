@@ -3,9 +3,10 @@
 //   y[m, n] = sum_k x[m, k] * s[n, k / group] * (nibble[n, k] - 8)
 //
 // Layout.  Weights are kept in the order in which the matrix units take them: a block of 16 outputs x 64 inputs is 512
-// bytes, 16 a lane; word s of a lane holds its four operand registers of inputs 16s .. 16s + 15, nibble i the first and
-// nibble i + 4 the second value of register i.  Scales lie as [16 outputs][group][output g and g + 8].  Outputs are padded to
-// 16 with scale 0, inputs to 64 with value 0.
+// bytes, 16 a lane; word s of lane (g, t) holds its four operand registers of multiplication s, nibble i the first and nibble
+// i + 4 the second value of register i: outputs g and g + 8, inputs 32 (s / 2) + 8t + 4 (s % 2) .. + 3.  (The order of the inputs
+// is free as long as both operands share it: with this one a lane's inputs of x are neighbours.)  Scales lie as [16 outputs]
+// [group][output g and g + 8].  Outputs are padded to 16 with scale 0, inputs to 64 with value 0.
 //
 // Arithmetic.  The weights are exact as bfloat16: a nibble is dropped into the mantissa of 128 and 136 subtracted (4
 // instructions for 4 values).  Activations are fp32 and enter as three bfloat16 planes each, x = hi + mid + lo exactly (24
@@ -64,7 +65,7 @@ __global__ void __launch_bounds__(256) q4_pack_kernel(const uint8_t* packed, uin
         for (int s = 0; s < 4; ++s) {
             w[s] = 0;
             for (int i = 0; i < 4; ++i) {
-                const int n = nt * 16 + g + 8 * (i & 1), k = kb * 64 + s * 16 + 2 * t + 8 * (i >> 1);
+                const int n = nt * 16 + g + 8 * (i & 1), k = kb * 64 + (s >> 1) * 32 + 8 * t + 4 * (s & 1) + 2 * (i >> 1);
                 w[s] |= (uint32_t)nibble_of(packed, K, N, n, k) << (4 * i) | (uint32_t)nibble_of(packed, K, N, n, k + 1) << (4 * i + 16);
             }
         }
@@ -78,9 +79,9 @@ __global__ void __launch_bounds__(256) q4_unpack_kernel(const uint4* q, uint8_t*
         const int n = (int)(x / bytes), j = (int)(x - n * bytes);
         int v = 0;
         for (int h = 0; h < 2; ++h) {
-            const int k = 2 * j + h, g = n & 7, kk = k & 15, t = (kk & 7) >> 1, i = ((n >> 3) & 1) + 2 * (kk >> 3);
+            const int k = 2 * j + h, g = n & 7, t = (k & 31) >> 3, s = 2 * ((k & 63) >> 5) + ((k & 7) >> 2), i = ((n >> 3) & 1) + 2 * ((k & 3) >> 1);
             const uint32_t* w = reinterpret_cast<const uint32_t*>(q + ((size_t)(n >> 4) * kbs + (k >> 6)) * 32 + g * 4 + t);
-            v |= (k < K ? (w[(k & 63) >> 4] >> (4 * i + 16 * (k & 1))) & 15 : 8) << (4 * h);
+            v |= (k < K ? (w[s] >> (4 * i + 16 * (k & 1))) & 15 : 8) << (4 * h);
         }
         packed[x] = (uint8_t)v;
     }
@@ -195,11 +196,19 @@ __global__ void __launch_bounds__(THREADS, C::MT == 0 ? (C::NT == 1 ? 3 : 2) : 1
     asm volatile("griddepcontrol.wait;" ::: "memory");                 // x may come from the kernel ahead, y may be read by it
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
 
-    const bool even = (a.K & 1) == 0;
-    // inputs k and k + 1 of a row; zeros behind the last input
-    auto pair_at = [&](const float* row, int k, bool whole) {
-        if (whole) return __ldcg(reinterpret_cast<const float2*>(row + k));
-        return make_float2(k < a.K ? __ldcg(row + k) : 0.0f, k + 1 < a.K ? __ldcg(row + k + 1) : 0.0f);
+    // inputs k .. k + 3 of a row (k a multiple of four); zeros behind the last input
+    const bool by_16 = (a.K & 3) == 0;
+    auto four_at = [&](const float* row, int k) {
+        float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+        if (by_16) {
+            if (k < a.K) v = __ldcg(reinterpret_cast<const float4*>(row + k));
+        } else {
+            if (k < a.K) v.x = __ldcg(row + k);
+            if (k + 1 < a.K) v.y = __ldcg(row + k + 1);
+            if (k + 2 < a.K) v.z = __ldcg(row + k + 2);
+            if (k + 3 < a.K) v.w = __ldcg(row + k + 3);
+        }
+        return v;
     };
     if constexpr (MT == 0) {
         // Column plane * rows + row of a multiplication; the other columns' sums are not looked at, they take the last one's.
@@ -208,12 +217,10 @@ __global__ void __launch_bounds__(THREADS, C::MT == 0 ? (C::NT == 1 ? 3 : 2) : 1
         const float* row = x + (size_t)m * a.K;
 #pragma unroll 2
         for (int s = kb0 * 4 + first; s < kb1 * 4; s += per) {
-            const int k = s * 16 + 2 * t;
-            const bool whole = even && s * 16 + 16 <= a.K;
-            const float2 v0 = pair_at(row, k, whole), v1 = pair_at(row, k + 8, whole);
+            const float4 v = four_at(row, (s >> 1) * 32 + 8 * t + 4 * (s & 1));
             uint32_t p0[3], p1[3];
-            planes(v0.x, v0.y, p0);
-            planes(v1.x, v1.y, p1);
+            planes(v.x, v.y, p0);
+            planes(v.z, v.w, p1);
 #pragma unroll
             for (int p = 0; p < 3; ++p)
                 *reinterpret_cast<uint2*>(xs + ((size_t)(s >> 1) * 3 * rows + p * rows + m) * 64 + t * 16 + (s & 1) * 8) = make_uint2(p0[p], p1[p]);
@@ -225,19 +232,12 @@ __global__ void __launch_bounds__(THREADS, C::MT == 0 ? (C::NT == 1 ? 3 : 2) : 1
     constexpr int AHEAD = C::AHEAD, VN = AHEAD + 1;
     const float* xrow[TM];
 #pragma unroll
-    for (int mt = 0; mt < TM; ++mt) xrow[mt] = x + (size_t)min(mt * 8 + g, rows - 1) * a.K + 2 * t;      // rows behind the last: not stored
-    float2 v[VN][4];
-    auto load_step = [&](float2(&to)[4], int kb, int step) {
-        const int h = step / TM, mt = step - h * TM, k = kb * 64 + h * 32;
-        const bool whole = even && kb * 64 + 64 <= a.K;
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            if (whole) to[i] = __ldcg(reinterpret_cast<const float2*>(xrow[mt] + k + i * 8));
-            else {
-                const int at = k + i * 8 + 2 * t;
-                to[i] = make_float2(at < a.K ? __ldcg(xrow[mt] + k + i * 8) : 0.0f, at + 1 < a.K ? __ldcg(xrow[mt] + k + i * 8 + 1) : 0.0f);
-            }
-        }
+    for (int mt = 0; mt < TM; ++mt) xrow[mt] = x + (size_t)min(mt * 8 + g, rows - 1) * a.K;      // rows behind the last: not stored
+    float4 v[VN][2];
+    auto load_step = [&](float4(&to)[2], int kb, int step) {
+        const int h = step / TM, mt = step - h * TM, k = kb * 64 + h * 32 + 8 * t;
+        to[0] = four_at(xrow[mt], k);
+        to[1] = four_at(xrow[mt], k + 4);
     };
     if constexpr (MT > 0)
         if (kb0 < kb1) {
@@ -321,8 +321,8 @@ __global__ void __launch_bounds__(THREADS, C::MT == 0 ? (C::NT == 1 ? 3 : 2) : 1
                         }
                     }
                     uint32_t b[4][3];
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) planes(v[s % VN][i].x, v[s % VN][i].y, b[i]);
+                    const float4 u0 = v[s % VN][0], u1 = v[s % VN][1];
+                    planes(u0.x, u0.y, b[0]), planes(u0.z, u0.w, b[1]), planes(u1.x, u1.y, b[2]), planes(u1.z, u1.w, b[3]);
 #pragma unroll
                     for (int i = 0; i < NT; ++i) {
                         float c[4];
@@ -343,8 +343,8 @@ __global__ void __launch_bounds__(THREADS, C::MT == 0 ? (C::NT == 1 ? 3 : 2) : 1
                 if constexpr (R != 0) {
                     static_assert(AHEAD == 2, "two of three places to move");
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        const float2 w0 = v[R][i], w1 = v[(R + 1) % VN][i];
+                    for (int i = 0; i < 2; ++i) {
+                        const float4 w0 = v[R][i], w1 = v[(R + 1) % VN][i];
                         v[0][i] = w0, v[1][i] = w1;
                     }
                 }
