@@ -28,7 +28,7 @@
 extern "C" {
 #endif
 
-#define SHAINET_ATTN_VERSION 101
+#define SHAINET_ATTN_VERSION 102
 
 #define SHAINET_ATTN_OK 0
 #define SHAINET_ATTN_E_INVALID (-1)      /* bad argument / shape / null pointer / misaligned pointer */
@@ -418,9 +418,12 @@ int shainet_attn_paged_destroy(shainet_attn_paged* paged);
  * lens[r] == 0 is a padded row: nothing is written into pages, its out row is zeros.  Lengths are read on the device, so
  * the call can be captured and replayed as requests grow.  A length that the table cannot hold makes a row of zeros, a
  * table cell outside the pool is not followed (that request's out row is then unspecified); either is reported as
- * SHAINET_ATTN_E_INVALID by the next blocking call on ctx after the stream was synchronised.  Rows of pages behind a
- * request's last position are never used, whatever they hold.  Arithmetic is fp32 or better over the rows as the pages
- * hold them; results do not depend on what else is in the batch than through the split of a request's positions. */
+ * SHAINET_ATTN_E_INVALID by the next blocking call on ctx after the stream was synchronised (what the call of one request
+ * reports does not touch the others).  Rows of pages behind a request's last position are never used, whatever they
+ * hold; projections and rows that a request sees are finite (one that is not makes that request's outputs NaN).  Sums
+ * and softmax statistics are fp32; 16-bit rows are multiplied exactly, fp32 rows with operands rounded to 22 bits (2^-23),
+ * as exact as a plain fp32 loop over them.  The batch changes a result only through where a request's positions are
+ * split.  No log-sum-exp values are written (set_lse_out) and no peers are served (comm_set_target). */
 int shainet_attn_paged_decode_dev(shainet_attn_ctx* ctx, shainet_attn_paged* paged, const shainet_attn_kv* kv,
                                   void* k_pages, void* v_pages, int num_pages, const float* q_dev, const float* k_new_dev,
                                   const float* v_new_dev, float* out_dev, const int32_t* block_table, int table_width,
@@ -442,7 +445,9 @@ int shainet_attn_paged_gather_dev(shainet_attn_ctx* ctx, shainet_attn_paged* pag
  * q4_create quantises an fp32 matrix [K, N] as the Q8_0 one does: scale = max|w| / 7 (1 for an all-zero group), value =
  * round(w * (1 / scale)), ties to even.  create_raw takes host arrays, create_dev device arrays (read on the context's
  * stream before it returns).  All of them lay the nibbles out anew for the kernel.
- * y[rows, N] = x[rows, K] . dequant(W), fp32 sums of exact products; x is not rounded. */
+ * y[rows, N] = x[rows, K] . dequant(W), fp32 sums of exact products; x is not rounded.  x and y do not overlap.  A value
+ * of x that is not finite makes its row's outputs not finite and leaves the other rows alone.  Any stream, several at
+ * once; nothing is allocated by a product.  The caller synchronises its streams before q4_destroy. */
 typedef struct shainet_attn_q4 shainet_attn_q4;
 int shainet_attn_q4_create(shainet_attn_ctx* ctx, shainet_attn_q4** out, const float* w_host, int K, int N, int group);
 int shainet_attn_q4_create_raw(shainet_attn_ctx* ctx, shainet_attn_q4** out, const uint8_t* packed_host,
