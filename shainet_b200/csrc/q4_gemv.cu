@@ -146,7 +146,6 @@ struct Cfg {
     static constexpr int PLACE = KU * 640;                            // one block of outputs: 512 bytes a block of inputs, then scales
     static constexpr int UNIT = NT * PLACE;
     static constexpr int RING = MT == 0 ? 2 : NT == 1 ? 5 : 3;        // places of a warp's ring: one in use
-    static constexpr int AHEAD = MT <= 3 ? 2 : 1;                     // steps of x that are fetched ahead
     static constexpr int COLS = MT == 0 ? 8 : 8 * MT;                 // columns of the sums: planes and rows, or rows
     static constexpr int RED = COLS + 2;                              // floats between outputs in the sums' meeting place
     static constexpr int SET = WARPS * NT * 16 * RED;                 // floats of a set's sums
@@ -168,7 +167,8 @@ __global__ void __launch_bounds__(THREADS, C::MT == 0 ? (C::NT == 1 ? 3 : 2) : 1
     const float* x = a.x + (size_t)m0 * a.K;
 
     // ---- copies: for every set of this CTA the blocks of the warp's slice ----
-    int ld_set = blockIdx.x, ld_kb = kb0;
+    const int turned = MT > 0 && kb0 < kb1 ? kb0 + blockIdx.x % (kb1 - kb0) : kb0;
+    int ld_set = blockIdx.x, ld_kb = turned;
     uint32_t fill = 0;
     const uint32_t ring_at = static_cast<uint32_t>(__cvta_generic_to_shared(ring)) + lane * 16;
     auto fetch = [&]() {
@@ -187,7 +187,8 @@ __global__ void __launch_bounds__(THREADS, C::MT == 0 ? (C::NT == 1 ? 3 : 2) : 1
             }
             fill = fill == (C::RING - 1) * C::UNIT ? 0 : fill + C::UNIT;
             ld_kb += cnt;
-            if (ld_kb == kb1) ld_kb = kb0, ld_set += gridDim.x;
+            if (ld_kb == kb1) ld_kb = kb0;
+            if (ld_kb == turned) ld_set += gridDim.x;
         }
         copy_commit();
     };
@@ -228,8 +229,9 @@ __global__ void __launch_bounds__(THREADS, C::MT == 0 ? (C::NT == 1 ? 3 : 2) : 1
         __syncwarp();
     }
 
-    // More rows: x is fetched AHEAD steps (of eight rows and 32 inputs) ahead, straight from L2
-    constexpr int AHEAD = C::AHEAD, VN = AHEAD + 1;
+    // More rows: x is fetched AHEAD steps (of eight rows and 32 inputs) ahead, straight from L2.  CTAs start at different
+    // blocks of their slices: all at the same one would ask the same lines of L2 at the same time (2 %).
+    constexpr int AHEAD = 2, VN = AHEAD + 1;
     const float* xrow[TM];
 #pragma unroll
     for (int mt = 0; mt < TM; ++mt) xrow[mt] = x + (size_t)min(mt * 8 + g, rows - 1) * a.K;      // rows behind the last: not stored
@@ -241,8 +243,8 @@ __global__ void __launch_bounds__(THREADS, C::MT == 0 ? (C::NT == 1 ? 3 : 2) : 1
     };
     if constexpr (MT > 0)
         if (kb0 < kb1) {
-            load_step(v[0], kb0, 0);
-            if constexpr (AHEAD == 2) load_step(v[1], kb0, 1);
+            load_step(v[0], turned, 0);
+            load_step(v[1], turned, 1);
         }
 
     uint32_t take = 0;
@@ -257,7 +259,8 @@ __global__ void __launch_bounds__(THREADS, C::MT == 0 ? (C::NT == 1 ? 3 : 2) : 1
 #pragma unroll
                 for (int c = 0; c < 4; ++c) total[i][mt][c] = 0.0f;
 #pragma unroll 1
-        for (int kb = kb0; kb < kb1; kb += KU) {
+        for (int at = kb0; at < kb1; at += KU) {
+            const int kb = MT == 0 ? at : turned + at - kb0 < kb1 ? turned + at - kb0 : turned + at - kb1;
             copy_wait<C::RING - 2>();
             __syncwarp();
             fetch();                                                   // into the place that the last turn was done with
@@ -341,7 +344,6 @@ __global__ void __launch_bounds__(THREADS, C::MT == 0 ? (C::NT == 1 ? 3 : 2) : 1
                 // what is under way for the next block stands where that one looks for it
                 constexpr int R = 2 * MT % VN;
                 if constexpr (R != 0) {
-                    static_assert(AHEAD == 2, "two of three places to move");
 #pragma unroll
                     for (int i = 0; i < 2; ++i) {
                         const float4 w0 = v[R][i], w1 = v[(R + 1) % VN][i];
