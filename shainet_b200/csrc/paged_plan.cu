@@ -134,7 +134,7 @@ __global__ void __launch_bounds__(PLAN_THREADS) paged_plan_kernel(PagedPlanArgs 
     if (ctas > 1)
         asm volatile("barrier.cluster.arrive.aligned;\n barrier.cluster.wait.aligned;" ::: "memory");
 
-    const int t0 = rank * T + tid, step = ctas * T;
+    const unsigned t0 = rank * T + tid, step = ctas * T;               // unsigned: the last step may pass 2^31
     const bool ok = code == PLAN_OK;
     if (t0 == 0) {
         a.status[0] = code;
@@ -142,12 +142,12 @@ __global__ void __launch_bounds__(PLAN_THREADS) paged_plan_kernel(PagedPlanArgs 
         a.free_count_out[0] = ok ? (int)left : f;
         a.first[R] = ok ? (int)total.tokens : 0;
     }
-    for (int r = t0; r < R; r += step) {
+    for (unsigned r = t0; r < R; r += step) {
         a.lens_out[r] = s_len[r] + (ok ? s_delta[r] : 0);
         a.first[r] = ok ? s_new[r] : 0;
     }
     if (!ok) {
-        for (int t = t0; t < a.max_tokens; t += step) a.slots[t] = -1;
+        for (unsigned t = t0; t < a.max_tokens; t += step) a.slots[t] = -1;
         return;
     }
     // the k-th freed page
@@ -160,12 +160,12 @@ __global__ void __launch_bounds__(PLAN_THREADS) paged_plan_kernel(PagedPlanArgs 
         const int at = f + freed - 1 - i;
         return at < f ? a.free_pages[at] : freed_page(at - f);
     };
-    for (int k = t0; k < freed; k += step) a.free_pages[f + k] = freed_page(k);
-    for (int i = t0; i < total.grow; i += step) {
+    for (unsigned k = t0; k < freed; k += step) a.free_pages[f + k] = freed_page(k);
+    for (unsigned i = t0; i < total.grow; i += step) {
         const int r = owner_of(s_grow, R, i);
         a.block_table[(size_t)r * a.table_width + pages_of(s_len[r], a.by_page, P) + i - s_grow[r]] = popped_page(i);
     }
-    for (int t = t0; t < a.max_tokens; t += step) {
+    for (unsigned t = t0; t < a.max_tokens; t += step) {
         int slot = -1;
         if (t < total.tokens) {
             const int r = owner_of(s_new, R, t);

@@ -172,6 +172,29 @@ def test_steps_that_cannot_be_taken_change_nothing(ctx, what, tokens):
         assert check(ctx, lens, delta, table, P, free, count, tokens, in_place=in_place)[0] == want
 
 
+def test_the_longest_slot_map(ctx):
+    """2^31 - 1 places for slots: the last step of the loop that fills them passes 2^31."""
+    import torch
+    import shainet_b200 as S
+    if torch.cuda.mem_get_info()[0] < 24 << 30:
+        pytest.skip("needs 24 GB")
+    tokens = 2**31 - 1
+    dev = lambda *x: torch.tensor(x, dtype=torch.int32, device="cuda")
+    lens, delta, table, free, count, first, status = dev(15), dev(3), dev(4, -7), dev(9, 8, -9), dev(2), dev(-5, -5), dev(-5, -5)
+    slots = torch.full((tokens + 8192,), -5, dtype=torch.int32, device="cuda")      # no guard before it: the front is checked too
+    for page_rows, left in ((16, 1), (17, 1)):
+        lens.fill_(page_rows - 1)
+        count.fill_(2)
+        slots.fill_(-5)
+        torch.cuda.synchronize()
+        S.plan_pages_dev(ctx, 1, lens.data_ptr(), delta.data_ptr(), table.data_ptr(), 2, page_rows, free.data_ptr(), 3, count.data_ptr(),
+                         lens.data_ptr(), count.data_ptr(), first.data_ptr(), slots.data_ptr(), tokens, status.data_ptr())
+        ctx.sync()
+        assert status.tolist() == [OK, 0] and lens.item() == page_rows + 2 and count.item() == left and table.tolist() == [4, 8]
+        assert slots[:3].tolist() == [4 * page_rows + page_rows - 1, 8 * page_rows, 8 * page_rows + 1]
+        assert bool((slots[3:tokens] == -1).all()) and bool((slots[tokens:] == -5).all())
+
+
 def test_no_requests_and_no_tokens(ctx):
     free = np.arange(4, dtype=np.int32)
     empty = np.zeros(0, np.int32)
