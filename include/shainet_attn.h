@@ -387,7 +387,7 @@ int shainet_attn_decode_noalloc(const float* q_dev, const float* k_cache_dev, co
  * by their place in its table; then requests that grow pop theirs in the order of the requests, by place in the table.
  * Written: the new table cells, the stack, lens_out = lens + delta, free_count_out, first [requests + 1] (the exclusive
  * sums of max(delta, 0): where a request's new tokens start), slots [max_tokens] (the slot of every new token, -1 behind
- * the last one) and status [2].  Table cells and stack entries that are not in use keep what they held.  lens_out may be
+ * the last one and for a page outside the pool) and status [2].  Table cells and stack entries that are not in use keep what they held.  lens_out may be
  * lens and free_count_out may be free_count (a captured step advances its own state); no other two arrays may overlap.
  * Nothing is changed (lens_out = lens, free_count_out = free_count, first 0, slots -1) and status[0] is not 0 where
  * the step cannot be taken: SHORT, status[1] pages are missing; LENGTH, request status[1] has a length below 0 or above

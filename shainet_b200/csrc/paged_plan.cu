@@ -171,7 +171,7 @@ __global__ void __launch_bounds__(PLAN_THREADS) paged_plan_kernel(PagedPlanArgs 
             const int r = owner_of(s_new, R, t);
             const int pos = s_len[r] + (t - s_new[r]), col = divide(pos, a.by_page), before = pages_of(s_len[r], a.by_page, P);
             const int page = col < before ? a.block_table[(size_t)r * a.table_width + col] : popped_page(s_grow[r] + col - before);
-            slot = (int)((long long)page * P + (pos - col * P));
+            if (page_in_pool(page, a.num_pages)) slot = page * P + (pos - col * P);     // else: not a slot of another page
         }
         a.slots[t] = slot;
     }

@@ -172,6 +172,17 @@ def test_steps_that_cannot_be_taken_change_nothing(ctx, what, tokens):
         assert check(ctx, lens, delta, table, P, free, count, tokens, in_place=in_place)[0] == want
 
 
+def test_pages_outside_the_pool_have_no_slots(ctx):
+    """A table cell or a free page that is not a page: its slots are -1, also where page * page_rows would wrap to a slot
+    of the pool; the rest of the step is taken."""
+    P, NP = 16, 6
+    lens, delta = np.array([5, 20, 16, 3], np.int32), np.array([2, 1, 2, 2], np.int32)
+    table, free = np.array([[1 << 28, -7], [0, 1], [2, -7], [-1, -7]], np.int32), np.array([3, 4, NP, -9, -9, -9], np.int32)
+    status, _, count, tab, _, first, slots = device_plan(ctx, lens, delta, table, P, free, 3, 12)
+    assert status == [OK, 0] and count == 2 and list(first) == [0, 2, 3, 5, 7] and tab[2, 1] == NP
+    assert list(slots) == [-1, -1, 20, -1, -1, -1, -1] + [-1] * 5
+
+
 def test_the_longest_slot_map(ctx):
     """2^31 - 1 places for slots: the last step of the loop that fills them passes 2^31."""
     import torch
@@ -180,18 +191,19 @@ def test_the_longest_slot_map(ctx):
         pytest.skip("needs 24 GB")
     tokens = 2**31 - 1
     dev = lambda *x: torch.tensor(x, dtype=torch.int32, device="cuda")
-    lens, delta, table, free, count, first, status = dev(15), dev(3), dev(4, -7), dev(9, 8, -9), dev(2), dev(-5, -5), dev(-5, -5)
+    lens, delta, table, count, first, status = dev(15), dev(3), dev(4, -7), dev(2), dev(-5, -5), dev(-5, -5)
     slots = torch.full((tokens + 8192,), -5, dtype=torch.int32, device="cuda")      # no guard before it: the front is checked too
-    for page_rows, left in ((16, 1), (17, 1)):
+    for page_rows, left, pages in ((16, 1, 3), (17, 1, 3), (16, 1, 10)):     # pages 4, 8 and 9: outside a pool of three
+        free = dev(9, 8, *[-9] * (pages - 2))
         lens.fill_(page_rows - 1)
         count.fill_(2)
         slots.fill_(-5)
         torch.cuda.synchronize()
-        S.plan_pages_dev(ctx, 1, lens.data_ptr(), delta.data_ptr(), table.data_ptr(), 2, page_rows, free.data_ptr(), 3, count.data_ptr(),
+        S.plan_pages_dev(ctx, 1, lens.data_ptr(), delta.data_ptr(), table.data_ptr(), 2, page_rows, free.data_ptr(), pages, count.data_ptr(),
                          lens.data_ptr(), count.data_ptr(), first.data_ptr(), slots.data_ptr(), tokens, status.data_ptr())
         ctx.sync()
         assert status.tolist() == [OK, 0] and lens.item() == page_rows + 2 and count.item() == left and table.tolist() == [4, 8]
-        assert slots[:3].tolist() == [4 * page_rows + page_rows - 1, 8 * page_rows, 8 * page_rows + 1]
+        assert slots[:3].tolist() == ([4 * page_rows + page_rows - 1, 8 * page_rows, 8 * page_rows + 1] if pages > 8 else [-1, -1, -1])
         assert bool((slots[3:tokens] == -1).all()) and bool((slots[tokens:] == -5).all())
 
 
