@@ -134,8 +134,6 @@ struct Cursor {
     __device__ __forceinline__ int place() const { return at + PAIR_COST + j; }
 };
 
-// A request's length; 0 where the table cannot hold it.
-__device__ __forceinline__ int valid_len(int len, int max_len) { return (unsigned)len <= (unsigned)max_len ? len : 0; }
 template <class C>
 __device__ __forceinline__ int tiles_of(int len) { return (int)(((unsigned)len + C::TW - 1) / C::TW); }
 
@@ -1122,7 +1120,7 @@ PagedPlan paged_decode_plan(const HeadShape& hs, int kv_elem_bytes, int sm_count
 }
 
 cudaError_t launch_paged_decode(PagedDecodeArgs a, const PagedPlan& p, float* workspace, unsigned* counters, cudaStream_t s) {
-    a.max_len = (int)std::min<long long>((long long)a.table_width * a.page_rows, 0x7fffffff);
+    a.max_len = max_len_of(a.table_width, a.page_rows);
     a.by_page = fast_div(a.page_rows);
     a.by_tiles = fast_div(p.head_tiles);
     a.head_tiles = p.head_tiles;

@@ -57,12 +57,6 @@ __device__ __forceinline__ int owner_of(const int* sums, int n, int x) {
     return lo;
 }
 
-// n / P rounded up
-__device__ __forceinline__ int pages_of(int n, FastDiv by, int page_rows) {
-    const int q = divide(n, by);
-    return q + (n > q * page_rows ? 1 : 0);
-}
-
 __device__ __forceinline__ Sums change_of(int len, int delta, FastDiv by, int page_rows) {
     const int before = pages_of(len, by, page_rows), after = pages_of(len + delta, by, page_rows);
     return {delta > 0 ? delta : 0, after > before ? after - before : 0, before > after ? before - after : 0};
@@ -180,7 +174,7 @@ __global__ void __launch_bounds__(PLAN_THREADS) paged_plan_kernel(PagedPlanArgs 
 }  // namespace
 
 cudaError_t launch_paged_plan(PagedPlanArgs a, cudaStream_t s) {
-    a.max_len = (int)std::min<long long>((long long)a.table_width * a.page_rows, 0x7fffffff);
+    a.max_len = max_len_of(a.table_width, a.page_rows);
     a.by_page = fast_div(a.page_rows);
     // one CTA up to 8 tokens and 2 requests a thread: a cluster's launch and barrier cost more than it saves there
     const bool wide = a.max_tokens > 8 * PLAN_THREADS || a.requests > 2 * PLAN_THREADS;

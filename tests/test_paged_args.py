@@ -105,10 +105,10 @@ _HOST = r"""
 #include "paged_index.h"
 using namespace shainet;
 extern "C" {
-int t_pages(long long n, int p) { return pages_for(n, p); }
+int t_pages(int n, int p) { return pages_of(n, fast_div(p), p); }
 int t_page(int page, int n) { return page_in_pool(page, n); }
 int t_slot(int slot, int n, int p) { return slot_in_pool(slot, n, p); }
-int t_len(int len, int w, int p) { return length_fits(len, w, p); }
+int t_len(int len, int w, int p) { return valid_len(len, max_len_of(w, p)); }
 int t_div(int n, int d) { return divide(n, fast_div(d)); }
 long long t_div_sweep(int d) {      // first n whose quotient is wrong, or -1: around every multiple up to 2^31 - 1, or a grid of them
     const FastDiv f = fast_div(d);
@@ -131,14 +131,13 @@ def test_index_arithmetic_keeps_bad_pages_out_and_64_bits(tmp_path):
     subprocess.run(["g++", "-std=c++17", "-O1", "-shared", "-fPIC", "-I", os.path.join(ROOT, "shainet_b200", "csrc"), str(src), "-o",
                     str(so)], check=True)
     L = C.CDLL(str(so))
-    L.t_pages.argtypes = [C.c_longlong, C.c_int]
     L.t_row.restype = C.c_ulonglong
     L.t_div_sweep.restype = C.c_longlong
     assert all(L.t_div_sweep(d) == -1 for d in [*range(1, 130), *range(131, 4097, 61), 4095, 4096])
     big = 2**31 - 1
-    assert [L.t_pages(n, 16) for n in (0, 1, 16, 17)] == [0, 1, 1, 2] and L.t_pages(big, 1) == big
+    assert [L.t_pages(n, 16) for n in (0, 1, 16, 17)] == [0, 1, 1, 2] and L.t_pages(big, 1) == big and L.t_pages(big, 4096) == 1 << 19
     assert [L.t_page(p, 5) for p in (-1, 0, 4, 5, big, -big)] == [0, 1, 1, 0, 0, 0]
     assert [L.t_slot(s, 5, 16) for s in (-1, 0, 79, 80, big)] == [0, 1, 1, 0, 0]
     assert L.t_slot(big, 1 << 20, 4096) == 1          # the product is taken in 64 bits
-    assert [L.t_len(n, 3, 16) for n in (-1, 0, 48, 49, big)] == [0, 1, 1, 0, 0] and L.t_len(big, 1 << 20, 4096) == 1
+    assert [L.t_len(n, 3, 16) for n in (-1, 0, 48, 49, big)] == [0, 0, 48, 0, 0] and L.t_len(big, 1 << 20, 4096) == big
     assert L.t_row(big - 1, 128, 127, 4096, 4095) == ((big - 1) * 128 + 127) * 4096 + 4095
