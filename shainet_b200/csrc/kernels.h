@@ -301,8 +301,11 @@ struct Q4GemvArgs {
     float* y;
     int M, N, K, group;
     int pass_rows;          // set by the launch: rows of one pass over the weights
+    AttnStatus* status;
 };
 cudaError_t launch_q4_gemv(const Q4GemvArgs& a, int sm_count, cudaStream_t s);
+// The same for several rows on the tensor cores; stored: groups per block of outputs in the layout.
+cudaError_t launch_q4_rows(const Q4GemvArgs& a, int stored, int sm_count, cudaStream_t s);
 
 // Sets the calling thread's message for shainet_attn_last_error().
 void set_last_error_message(const char* msg);

@@ -456,6 +456,7 @@ cudaError_t launch_group(Q4GemvArgs a, int sm_count, cudaStream_t s) {
 namespace shainet {
 
 cudaError_t launch_q4_gemv(const Q4GemvArgs& a, int sm_count, cudaStream_t s) {
+    if (a.M > 8) return launch_q4_rows(a, stored_groups(a.K, a.group), sm_count, s);
     return a.group == 32 ? launch_group<32>(a, sm_count, s) : a.group == 64 ? launch_group<64>(a, sm_count, s) : launch_group<128>(a, sm_count, s);
 }
 
@@ -623,6 +624,7 @@ int shainet_attn_q4_gemv_dev(shainet_attn_ctx* ctx, const shainet_attn_q4* w, co
     a.N = w->N;
     a.K = w->K;
     a.group = w->group;
+    a.status = ctx->status_dev;
     ctx->last_fused = false;
     CU(launch_q4_gemv(a, ctx->sm_count, stream ? (cudaStream_t)stream : ctx->stream));
     return SHAINET_ATTN_OK;
