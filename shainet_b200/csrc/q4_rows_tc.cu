@@ -100,10 +100,10 @@ struct Tile {
     static constexpr int TMEM_COLS = 512, TMEM_A = TMEM_COLS - 2 * A_SLOTS * A_COLS;
     static constexpr int DH = TMEM_A / D_COLS >= 4 ? 2 : 1;      // sums of each half
     static constexpr int NB = 4, B_BYTES = COLS * 128;           // stages of planes, 64 inputs each, 128-byte swizzle
-    static constexpr int NX = 4, X_BYTES = NT * 256;             // stages of fp32 rows
+    static constexpr int NX = NT <= 40 ? 3 : 2, X_BYTES = NT * 256;      // stages of fp32 rows, of two warpgroups
     static constexpr int NW = 6, W_BYTES = 1024;                 // stages of a converting warp: 32 outputs x 64 inputs
     static constexpr int NS = 8, S_BYTES = 128;                  // stages of an accumulating warp: a scale of 32 outputs
-    static constexpr int AT_X = NB * B_BYTES, AT_W = AT_X + NX * X_BYTES, AT_S = AT_W + 8 * NW * W_BYTES, AT_BARS = AT_S + 8 * NS * S_BYTES;
+    static constexpr int AT_X = NB * B_BYTES, AT_W = AT_X + 2 * NX * X_BYTES, AT_S = AT_W + 8 * NW * W_BYTES, AT_BARS = AT_S + 8 * NS * S_BYTES;
     static constexpr int BARS = 2 * NB + 4 * A_SLOTS + 4 * DH;
     static constexpr int USED = AT_BARS + BARS * 8 + 16;
     // Never two CTAs on an SM, nor another kernel that allocates tensor memory beside one: a cluster's CTA could wait for columns
@@ -132,7 +132,7 @@ template <class C>
 __global__ void __launch_bounds__(THREADS, 1) q4_rows_kernel(Q4GemvArgs a, int kbs, int stored, int blocks, int tiles) {
     constexpr int NT = C::NT, GB = C::GB, PARTS = C::PARTS, DH = C::DH, NB = C::NB;
     extern __shared__ __align__(1024) unsigned char qr_smem[];
-    uint64_t* b_full = reinterpret_cast<uint64_t*>(qr_smem + C::AT_BARS);      // NB: eight row warps
+    uint64_t* b_full = reinterpret_cast<uint64_t*>(qr_smem + C::AT_BARS);      // NB: four row warps
     uint64_t* b_free = b_full + NB;                                            // NB: both halves' multiplications
     uint64_t* a_full = b_free + NB;                                            // [half][slot]: four converting warps
     uint64_t* a_free = a_full + 2 * C::A_SLOTS;                                // [half][slot]: the multiplications
@@ -141,7 +141,7 @@ __global__ void __launch_bounds__(THREADS, 1) q4_rows_kernel(Q4GemvArgs a, int k
     uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(d_free + 2 * DH);
     const int warp = uniform_warp_index(), lane = threadIdx.x & 31, wg = warp >> 2, quad = warp & 3;
     if (threadIdx.x == 0) {
-        for (int i = 0; i < NB; ++i) mbar_init(&b_full[i], 8), mbar_init(&b_free[i], 2);
+        for (int i = 0; i < NB; ++i) mbar_init(&b_full[i], 4), mbar_init(&b_free[i], 2);
         for (int i = 0; i < 2 * C::A_SLOTS; ++i) mbar_init(&a_full[i], 4), mbar_init(&a_free[i], 1);
         for (int i = 0; i < 2 * DH; ++i) mbar_init(&d_full[i], 1), mbar_init(&d_free[i], 4);
         fence_mbar_init();
@@ -217,35 +217,42 @@ __global__ void __launch_bounds__(THREADS, 1) q4_rows_kernel(Q4GemvArgs a, int k
         if (warp == 0) multiply(std::integral_constant<int, 0>{});
         if (warp == 2) multiply(std::integral_constant<int, 1>{});
     } else if (wg < 3) {
-        // ---- rows: fp32 from L2 by asynchronous copies, every thread converts the pieces that it requested ----
+        // ---- rows: two warpgroups take blocks in turn; fp32 from L2 by asynchronous copies, every thread converts the pieces that
+        // it requested ----
         fewer_registers<48>();
-        constexpr int PIECES = (NT + 15) / 16;
-        const int tid = threadIdx.x - 128, c4 = tid & 15, t0 = tid >> 4;       // piece j: row t0 + 16 j, inputs 4 c4 .. + 3
+        constexpr int PIECES = NT / 8;
+        const int tid = threadIdx.x - wg * 128, c4 = tid & 15, t0 = tid >> 4;  // piece j: row t0 + 8 j, inputs 4 c4 .. + 3
         const bool by_16 = (a.K & 3) == 0;
-        const uint32_t raw = smem_u32(qr_smem + C::AT_X) + tid * 16;
+        const uint32_t raw = smem_u32(qr_smem + C::AT_X) + (wg - 1) * (C::NX * C::X_BYTES) + tid * 16;
+        const unsigned char* from = qr_smem + C::AT_X + (wg - 1) * (C::NX * C::X_BYTES) + tid * 16;
         const float* row = a.x + (size_t)(m0 + min(t0, rows - 1)) * a.K + c4 * 4;
-        const int pieces = t0 < rows ? (rows - t0 + 15) / 16 : 0;                // rows behind the last one: whatever stands in the stages
-        const size_t stride = (size_t)16 * a.K;
-        int ld = 0, ld_kb = kb0;
-        uint32_t fill = raw;
+        const int pieces = t0 < rows ? (rows - t0 + 7) / 8 : 0;                // rows behind the last one: whatever stands in the stages
+        const size_t stride = (size_t)8 * a.K;
+        const int slice = kb1 - kb0;
+        int ld = wg - 1, ld_kb = kb0 + (slice > 0 ? ld % slice : 0);
+        uint32_t fill = 0;
         auto fetch = [&]() {
             if (ld < total) {
-                const float* src = row + ld_kb * 64;
                 const int left = a.K - ld_kb * 64 - c4 * 4;                    // inputs of this piece; zeros behind the last
+                const float* src = left > 0 ? row + ld_kb * 64 : a.x;
+                const size_t by = left > 0 ? stride : 0;
                 if (by_16) {
                     const int bytes = left > 0 ? 16 : 0;
-                    if (left <= 0) src = a.x;
 #pragma unroll
-                    for (int j = 0; j < PIECES; ++j)
-                        if (j < pieces) copy16(fill + j * 4096, left > 0 ? src + j * stride : src, bytes);
+                    for (int j = 0; j < PIECES; ++j) {
+                        if (j >= pieces) break;
+                        copy16(raw + fill + j * 2048, src, bytes);
+                        src += by;
+                    }
                 } else {
 #pragma unroll 1
                     for (int j = 0; j < pieces; ++j)
-                        for (int e = 0; e < 4; ++e) copy4(fill + j * 4096 + e * 4, left > e ? src + j * stride + e : a.x, left > e ? 4 : 0);
+                        for (int e = 0; e < 4; ++e) copy4(raw + fill + j * 2048 + e * 4, left > e ? src + j * by + e : a.x, left > e ? 4 : 0);
                 }
-                fill = fill == raw + (C::NX - 1) * C::X_BYTES ? raw : fill + C::X_BYTES;
-                ++ld;
-                if (++ld_kb == kb1) ld_kb = kb0;
+                fill = fill == (C::NX - 1) * C::X_BYTES ? 0 : fill + C::X_BYTES;
+                ld += 2;
+                ld_kb += 2;
+                while (ld_kb >= kb1) ld_kb -= slice;
             }
             copy_commit();
         };
@@ -253,31 +260,27 @@ __global__ void __launch_bounds__(THREADS, 1) q4_rows_kernel(Q4GemvArgs a, int k
         asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
 #pragma unroll 1
         for (int i = 0; i < C::NX - 1; ++i) fetch();
-        Ring<NB> rb;
         uint32_t take = 0;
 #pragma unroll 1
-        for (int n = 0; n < total; ++n) {
+        for (int n = wg - 1; n < total; n += 2) {
             copy_wait<C::NX - 2>();
             fetch();                                                           // over what this thread converted last
-            if (!mbar_wait(&b_free[rb.slot], rb.parity ^ 1u, a.status, 93)) break;
-            unsigned char* stage = qr_smem + rb.slot * C::B_BYTES + (c4 & 1) * 8;
+            const int slot = n & (NB - 1);
+            if (!mbar_wait(&b_free[slot], (uint32_t)(n / NB & 1) ^ 1u, a.status, 93)) break;
+            unsigned char* stage = qr_smem + slot * C::B_BYTES + t0 * 128 + (((c4 >> 1) ^ t0) << 4) + (c4 & 1) * 8;
 #pragma unroll
             for (int j = 0; j < PIECES; ++j) {
                 if (j >= pieces) break;
-                const float4 v = *reinterpret_cast<const float4*>(qr_smem + C::AT_X + take + tid * 16 + j * 4096);
+                const float4 v = *reinterpret_cast<const float4*>(from + take + j * 2048);
                 uint32_t p0[3], p1[3];
                 planes(v.x, v.y, p0);
                 planes(v.z, v.w, p1);
 #pragma unroll
-                for (int p = 0; p < 3; ++p) {
-                    const int r = p * NT + t0 + 16 * j;                        // r & 7 == t0 & 7
-                    *reinterpret_cast<uint2*>(stage + r * 128 + (((c4 >> 1) ^ (t0 & 7)) << 4)) = make_uint2(p0[p], p1[p]);
-                }
+                for (int p = 0; p < 3; ++p) *reinterpret_cast<uint2*>(stage + (p * NT + 8 * j) * 128) = make_uint2(p0[p], p1[p]);
             }
             fence_proxy_async_smem();
             __syncwarp();
-            if (lane == 0) mbar_arrive(&b_full[rb.slot]);
-            rb.next();
+            if (lane == 0) mbar_arrive(&b_full[slot]);
             take = take == (C::NX - 1) * C::X_BYTES ? 0 : take + C::X_BYTES;
         }
         copy_wait<0>();
