@@ -43,7 +43,7 @@ namespace {
 
 constexpr unsigned FULL = 0xffffffffu;
 constexpr int WARPS = 8, THREADS = WARPS * 32;
-constexpr int MAX_MT = 5;               // rows of eight in one pass
+constexpr int MAX_MT = 3;               // rows of eight, all in one pass over the weights
 constexpr int SMEM_MAX = 220 * 1024;
 
 int blocks_of(int n, int d) { return (n + d - 1) / d; }
@@ -163,8 +163,7 @@ __global__ void __launch_bounds__(THREADS, C::MT == 0 ? (C::NT == 1 ? 3 : 2) : 1
     unsigned char* xs = q4_smem + C::FIXED;                            // MT = 0: [pairs of 16 inputs][column][t][2 x 8 bytes]
     const int slice = ((kbs + WARPS - 1) / WARPS + C::EVEN - 1) / C::EVEN * C::EVEN, kb0 = min(warp * slice, kbs), kb1 = min(kb0 + slice, kbs);
     const int sets = (blocks + NT - 1) / NT;                           // of NT blocks of 16 outputs
-    const int m0 = blockIdx.y * a.pass_rows, rows = min(a.pass_rows, a.M - m0);
-    const float* x = a.x + (size_t)m0 * a.K;
+    const int rows = a.M;
 
     // ---- copies: for every set of this CTA the blocks of the warp's slice ----
     const int turned = MT > 0 && kb0 < kb1 ? kb0 + blockIdx.x % (kb1 - kb0) : kb0;
@@ -215,7 +214,7 @@ __global__ void __launch_bounds__(THREADS, C::MT == 0 ? (C::NT == 1 ? 3 : 2) : 1
         // Column plane * rows + row of a multiplication; the other columns' sums are not looked at, they take the last one's.
         // A lane makes the three planes of four inputs: eight steps of 16 inputs at a time, or four of both rows.
         const int per = rows == 1 ? 8 : 4, m = rows == 1 ? 0 : g & 1, first = rows == 1 ? g : g >> 1;
-        const float* row = x + (size_t)m * a.K;
+        const float* row = a.x + (size_t)m * a.K;
 #pragma unroll 2
         for (int s = kb0 * 4 + first; s < kb1 * 4; s += per) {
             const float4 v = four_at(row, (s >> 1) * 32 + 8 * t + 4 * (s & 1));
@@ -234,7 +233,7 @@ __global__ void __launch_bounds__(THREADS, C::MT == 0 ? (C::NT == 1 ? 3 : 2) : 1
     constexpr int AHEAD = 2, VN = AHEAD + 1;
     const float* xrow[TM];
 #pragma unroll
-    for (int mt = 0; mt < TM; ++mt) xrow[mt] = x + (size_t)min(mt * 8 + g, rows - 1) * a.K;      // rows behind the last: not stored
+    for (int mt = 0; mt < TM; ++mt) xrow[mt] = a.x + (size_t)min(mt * 8 + g, rows - 1) * a.K;      // rows behind the last: not stored
     float4 v[VN][2];
     auto load_step = [&](float4(&to)[2], int kb, int step) {
         const int h = step / TM, mt = step - h * TM, k = kb * 64 + h * 32 + 8 * t;
@@ -377,7 +376,7 @@ __global__ void __launch_bounds__(THREADS, C::MT == 0 ? (C::NT == 1 ? 3 : 2) : 1
                         const float* s = meet + (w * (NT * 16) + n) * C::RED + m;
                         sum += s[2 * rows] + s[rows] + s[0];
                     }
-                    if (out < a.N) a.y[(size_t)(m0 + m) * a.N + out] = sum;
+                    if (out < a.N) a.y[(size_t)m * a.N + out] = sum;
                 }
             }
         } else {
@@ -387,7 +386,7 @@ __global__ void __launch_bounds__(THREADS, C::MT == 0 ? (C::NT == 1 ? 3 : 2) : 1
                 float sum = 0.0f;
 #pragma unroll
                 for (int w = 0; w < WARPS; ++w) sum += meet[(w * NT * 16 + n) * C::RED + m];
-                if (out < a.N) a.y[(size_t)(m0 + m) * a.N + out] = sum;
+                if (out < a.N) a.y[(size_t)m * a.N + out] = sum;
             }
             __syncthreads();
         }
@@ -411,10 +410,9 @@ cudaError_t launch(const Q4GemvArgs& a, int sm_count, cudaStream_t s) {
         if (e != cudaSuccess) return e;
         if (dev < 64) configured.fetch_or(1ull << dev, std::memory_order_release);
     }
-    const int passes = blocks_of(a.M, a.pass_rows);
     const int per_sm = MT == 0 ? std::max(1, std::min(NT == 1 ? 3 : 2, (int)(227 * 1024 / (smem + 1024)))) : 1;
     cudaLaunchConfig_t cfg{};
-    cfg.gridDim = dim3(std::min(sets, std::max(1, sm_count * per_sm / std::min(passes, per_sm))), passes);
+    cfg.gridDim = dim3(std::min(sets, sm_count * per_sm));
     cfg.blockDim = dim3(THREADS);
     cfg.dynamicSmemBytes = smem;
     cfg.stream = s;
@@ -430,25 +428,18 @@ template <int MT, int G>
 cudaError_t launch_rows(const Q4GemvArgs& a, int sm_count, cudaStream_t s) {
     // blocks of outputs that share the planes of x: four or two where that still leaves a CTA for most SMs (4096 x 4096, 16
     // rows: 24 us with one, 15 us with two; 8200 x 2048, 33 rows: 31 us with two, 21 us with four)
-    const long long work = (long long)blocks_of(a.N, 16) * blocks_of(a.M, a.pass_rows), most = sm_count * 3 / 4;
+    const long long work = blocks_of(a.N, 16), most = sm_count * 3 / 4;
     return work >= 4 * most ? launch<MT, 4, G>(a, sm_count, s) : work >= 2 * most ? launch<MT, 2, G>(a, sm_count, s) : launch<MT, 1, G>(a, sm_count, s);
 }
 
 template <int G>
-cudaError_t launch_group(Q4GemvArgs a, int sm_count, cudaStream_t s) {
-    a.pass_rows = a.M;
+cudaError_t launch_group(const Q4GemvArgs& a, int sm_count, cudaStream_t s) {
     if (a.M <= 2 && Cfg<0, 1, G>::FIXED + plane_bytes(a) <= SMEM_MAX) {
         // two blocks of outputs share the reads of x's planes where every CTA has several of them
         return blocks_of(a.N, 16) >= 8 * sm_count && Cfg<0, 2, G>::FIXED + plane_bytes(a) <= 112 * 1024 ? launch<0, 2, G>(a, sm_count, s) : launch<0, 1, G>(a, sm_count, s);
     }
-    a.pass_rows = blocks_of(a.M, blocks_of(a.M, 8 * MAX_MT));
-    switch (blocks_of(a.pass_rows, 8)) {
-        case 1: return launch_rows<1, G>(a, sm_count, s);
-        case 2: return launch_rows<2, G>(a, sm_count, s);
-        case 3: return launch_rows<3, G>(a, sm_count, s);
-        case 4: return launch_rows<4, G>(a, sm_count, s);
-        default: return launch_rows<5, G>(a, sm_count, s);
-    }
+    static_assert(MAX_MT == 3, "one instance for each");
+    return a.M <= 8 ? launch_rows<1, G>(a, sm_count, s) : a.M <= 16 ? launch_rows<2, G>(a, sm_count, s) : launch_rows<3, G>(a, sm_count, s);
 }
 
 }  // namespace
@@ -456,7 +447,13 @@ cudaError_t launch_group(Q4GemvArgs a, int sm_count, cudaStream_t s) {
 namespace shainet {
 
 cudaError_t launch_q4_gemv(const Q4GemvArgs& a, int sm_count, cudaStream_t s) {
-    if (a.M > 8) return launch_q4_rows(a, stored_groups(a.K, a.group), sm_count, s);
+    // The tensor cores of tcgen05 (us, here / there): from 25 rows on (700 x 900, 40 rows 6.8 / 5.5; 512 x 1000, 40 rows 4.3 / 4.6;
+    // 2048 x 8192, 33 rows 17.6 / 10.6); from nine on but for short sums into few outputs, which end before that kernel has
+    // filled its rings (16 rows: 512 x 1000 2.5 / 4.6, 1000 x 4000 4.6 / 4.7, 1500 x 400 5.0 / 4.6; 12 rows: 300 x 20000 8.8 / 5.0,
+    // 64 x 60000 14 / 8, 2048 x 8192 9.9 / 8.4); from three on where a warp's slice is long (8 rows: 2048 x 8192 5.7 / 8.2, 8192 x 2048 10.4 / 10.9,
+    // 11000 x 5000 33 / 18).
+    const bool small = a.K <= 1024 && a.N <= 8192 && a.K * a.N <= 4 << 20;
+    if (a.M > 8 * MAX_MT || (a.M > 8 && !small) || (a.M > 2 && a.K > 8192)) return launch_q4_rows(a, stored_groups(a.K, a.group), sm_count, s);
     return a.group == 32 ? launch_group<32>(a, sm_count, s) : a.group == 64 ? launch_group<64>(a, sm_count, s) : launch_group<128>(a, sm_count, s);
 }
 

@@ -526,7 +526,10 @@ cudaError_t launch(const Q4GemvArgs& a, int stored, int sm_count, cudaStream_t s
 
 template <int G>
 cudaError_t launch_group(Q4GemvArgs a, int stored, int sm_count, cudaStream_t s) {
-    const int passes = (a.M + 63) / 64;
+    // Up to 64 rows a pass over the weights; fewer where SMs would be idle (5000 x 100, 64 rows: 13.9 us with one pass, 7.5 with four).
+    int passes = (a.M + 63) / 64;
+    const long long ctas = (long long)((a.N + 255) / 256) * std::min(MAX_SPLITS, std::max(1, a.K / 256));
+    while (ctas * passes * 2 <= sm_count && a.M > 16 * passes) passes *= 2;
     a.pass_rows = (a.M + passes - 1) / passes;
     if (a.pass_rows <= 16) return launch<16, G>(a, stored, sm_count, s);
     if (a.pass_rows <= 32) return launch<32, G>(a, stored, sm_count, s);

@@ -65,6 +65,25 @@ def test_rows(ctx, K, N, M, group):
     W.close()
 
 
+# many tiles a CTA, blocks of inputs that end a group early, shared inputs of one to eight CTAs, one or more passes
+@pytest.mark.parametrize("group", [32, 64, 128])
+@pytest.mark.parametrize("K,N,M", [(200, 40001, 33), (64, 80000, 25), (449, 39000, 64), (2052, 38000, 12), (192, 257, 40), (320, 513, 64), (5000, 100, 64),
+                                   (4100, 4100, 24), (4097, 3900, 41), (12290, 300, 3), (9000, 5000, 8), (1000, 40, 1000), (1100, 900, 257)],
+                         ids=lambda v: str(v))
+def test_many_rows(ctx, K, N, M, group):
+    import torch
+    import shainet_b200 as S
+    rng = np.random.default_rng(K + N + M + group)
+    packed, scales = weights(rng, K, N, group)
+    x = rng.standard_normal((M, K)).astype(np.float32)
+    W = S.Q4Weight.from_quantized(ctx, packed, scales, K, group)
+    got = product(ctx, W, x, N)
+    ref = (torch.from_numpy(x).cuda().double() @ torch.from_numpy(dense(packed, scales, K, group)).cuda().T).cpu().numpy()
+    assert rel_err(got, ref) <= tol(K), rel_err(got, ref)
+    assert np.array_equal(got, product(ctx, W, x, N))
+    W.close()
+
+
 @pytest.mark.parametrize("group", [32, 64, 128])
 @pytest.mark.parametrize("K,N", [(1, 1), (2, 3), (31, 17), (32, 16), (33, 15), (63, 8), (65, 1), (127, 40), (129, 2), (255, 31), (513, 7), (2047, 100),
                                  (4097, 65), (12289, 24), (64, 20011)], ids=lambda v: str(v))
