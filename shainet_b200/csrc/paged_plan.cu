@@ -9,9 +9,10 @@
 // frees it, never in the stack cell that is being written, so nothing waits for a write of this launch.
 //
 // What bounds it is latency, not bytes (a few hundred KB at most): one round of loads, a scan over at most 8192 requests
-// that every CTA does for itself in shared memory, one or two dependent loads per output.  Large steps are spread over
-// one cluster of eight CTAs, whose barrier separates the reads of lens and free_count from the writes of lens_out and
-// free_count_out, which may be the same arrays; small ones take one CTA.
+// that every CTA does for itself in shared memory, one or two dependent loads per output.  Steps are spread over one cluster
+// of eight CTAs, whose barrier separates the reads of lens and free_count from the writes of lens_out and free_count_out,
+// which may be the same arrays; the smallest ones take one CTA.  Measured: 8 requests 2.7 us, 256 requests with
+// 15000 new tokens 6.1 us, of which an empty launch is 2.
 #include <algorithm>
 #include <atomic>
 #include "../../include/shainet_attn.h"
@@ -176,8 +177,10 @@ __global__ void __launch_bounds__(PLAN_THREADS) paged_plan_kernel(PagedPlanArgs 
 cudaError_t launch_paged_plan(PagedPlanArgs a, cudaStream_t s) {
     a.max_len = max_len_of(a.table_width, a.page_rows);
     a.by_page = fast_div(a.page_rows);
-    // one CTA up to 8 tokens and 2 requests a thread: a cluster's launch and barrier cost more than it saves there
-    const bool wide = a.max_tokens > 8 * PLAN_THREADS || a.requests > 2 * PLAN_THREADS;
+    // One CTA where a thread has one token or request at most, else the cluster (us, one / eight CTAs: 8 chats 2.7 / 2.9, 64
+    // requests and 960 tokens 5.0 / 4.5, 256 requests and 15000 tokens 8.3 / 6.1, 2000 requests 13.0 / 8.7).  256 threads a CTA for small steps,
+    // whose scan and barriers are shorter (8 chats 2.7, with 1024 threads 3.5).
+    const bool wide = a.max_tokens + (long long)a.requests > 256;
     const bool narrow = a.max_tokens <= 1024 && a.requests <= 256;
     const size_t smem = (size_t)a.requests * 5 * sizeof(int);
     static std::atomic<unsigned long long> configured{0};   // bit per device

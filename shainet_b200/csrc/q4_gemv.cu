@@ -13,12 +13,18 @@
 // bits cut into 8 + 8 + 8), so no operand is rounded.  m16n8k16 multiplications with fp32 accumulators; the sums of 32
 // or 64 inputs start from zero and are added in fp32 with their scale, so sums that the matrix units cut off stay short.
 //   * One or two rows: the planes are the columns of one multiplication (2 rows x 3 planes of 8).
-//   * More rows: eight rows a multiplication, three of them for the planes, up to 40 rows a pass over the weights.
+//   * Up to 24 rows: eight rows a multiplication, three of them for the planes.  More rows, and most products of more than
+//     eight, are taken by q4_rows_tc.cu.
 //
 // Work.  A CTA takes NT blocks of outputs at a time and splits their inputs over its eight warps, each with a ring of its own
-// in shared memory that asynchronous copies fill RING blocks ahead; the warps' sums meet in shared memory.  With one row
-// HBM bounds it (0.5 byte and 4 / group bytes a weight), with many the matrix units.  The first weights are requested
-// before the wait for the kernel ahead in the stream: they never depend on it.
+// in shared memory that asynchronous copies fill RING - 1 places ahead; the warps' sums meet in shared memory.  The first
+// weights are requested before the wait for the kernel ahead in the stream: they never depend on it.
+//
+// Bounds.  One row: 0.5 byte and 4 / group bytes a weight from HBM; the integer pipe is as busy (11 instructions for 8 nibbles):
+// 2048 -> 128256 in groups of 64 takes 30.6 us, 4.8 TB/s or 75 % of a copy's rate, with 53 % of the cycles of that pipe and 58 %
+// of the issue slots taken.  2048 -> 512 takes 2.2 us, a launch.  Several rows: the latency of eight warps an SM, whose rows come from L2 two steps
+// ahead (8 x 2048 -> 8192 5.8 us; one step ahead 6.4 % to 14 % longer from 17 rows on).  Fetching them by asynchronous copies into shared
+// memory was slower, and two scaled half-precision planes instead of three were not faster.
 #include <cuda_runtime.h>
 #include <math.h>
 #include <stdint.h>
@@ -426,8 +432,8 @@ cudaError_t launch(const Q4GemvArgs& a, int sm_count, cudaStream_t s) {
 
 template <int MT, int G>
 cudaError_t launch_rows(const Q4GemvArgs& a, int sm_count, cudaStream_t s) {
-    // blocks of outputs that share the planes of x: four or two where that still leaves a CTA for most SMs (4096 x 4096, 16
-    // rows: 24 us with one, 15 us with two; 8200 x 2048, 33 rows: 31 us with two, 21 us with four)
+    // blocks of outputs that share the planes of x: four or two where that still leaves a CTA for most SMs (us with one, two and
+    // four: 8 x 2048 -> 2048 3.8, 4.2, 5.5; 8 x 4096 -> 4096 10.8, 7.3, 9.7; 8 x 2048 -> 8192 11.3, 7.5, 5.7)
     const long long work = blocks_of(a.N, 16), most = sm_count * 3 / 4;
     return work >= 4 * most ? launch<MT, 4, G>(a, sm_count, s) : work >= 2 * most ? launch<MT, 2, G>(a, sm_count, s) : launch<MT, 1, G>(a, sm_count, s);
 }
@@ -435,7 +441,8 @@ cudaError_t launch_rows(const Q4GemvArgs& a, int sm_count, cudaStream_t s) {
 template <int G>
 cudaError_t launch_group(const Q4GemvArgs& a, int sm_count, cudaStream_t s) {
     if (a.M <= 2 && Cfg<0, 1, G>::FIXED + plane_bytes(a) <= SMEM_MAX) {
-        // two blocks of outputs share the reads of x's planes where every CTA has several of them
+        // two blocks of outputs share the reads of x's planes where every CTA has several of them (128256 outputs 32.9 us with one,
+        // 30.7 with two; 20000 and 40000 the same)
         return blocks_of(a.N, 16) >= 8 * sm_count && Cfg<0, 2, G>::FIXED + plane_bytes(a) <= 112 * 1024 ? launch<0, 2, G>(a, sm_count, s) : launch<0, 1, G>(a, sm_count, s);
     }
     static_assert(MAX_MT == 3, "one instance for each");

@@ -1,17 +1,24 @@
-// Products of several activation rows with 4-bit weights on the 5th-generation tensor cores (tcgen05), sm_100a; the layout and
-// the formula are those of q4_gemv.cu.
+// Products of several activation rows with 4-bit weights on the 5th-generation tensor cores (tcgen05), sm_100a; the formula and
+// the layout are those of q4_gemv.cu.
 //
 // A CTA computes 256 outputs of up to NT rows, as two halves of 128.  The weights are the A operand: a thread owns an
 // output, unpacks 64 of its nibbles at a time into bfloat16 (exact) and puts them into tensor memory.  The rows are the B
-// operand: fp32 values as three bfloat16 planes (exact), made in the CTA, stored side by side as 3 NT columns of one
-// multiplication.  The sums of a group (or of 32 or 64 inputs) start from zero in tensor memory; the accumulating warps, a
+// operand: fp32 values as three bfloat16 planes (exact), made in the CTA, side by side as 3 NT columns of one
+// multiplication.  The sums of 32 (groups of 32), 64 or 128 inputs start from zero in tensor memory; the accumulating warps, a
 // thread an output again, add the three columns of a row and multiply by the group's scale in fp32.
 //
-// Bounds.  A multiplication of 16 inputs takes 64 cycles for up to 128 columns (40 rows), 96 for 192 (64 rows); mma.sync
-// takes 8.5 cycles of a quarter SM for 16 outputs and eight columns, so 33 rows take it 3.4 times as long.
-//
 // Where there are fewer tiles than SMs, the CTAs of a cluster share a tile's inputs and add their sums through distributed
-// shared memory, in the order of their ranks.
+// shared memory, in the order of their ranks.  Rows are cut into more passes where SMs would be idle even so.
+//
+// Bounds.  A multiplication of 16 inputs takes 64 cycles for up to 128 columns (40 rows), 96 for 192 (64 rows): 512 or 768 cycles a
+// step of 64 inputs x 256 outputs.  A step takes 900 (12 rows), 1000 (33) and 1700 (64): the warps that unpack, make planes and
+// accumulate take two thirds of the issue slots and each of the three chains is nearly as long as a step (without the unpacking
+// 17 % less at 9 rows, with an eighth of the read-out 27 % less at 64, with an eighth of the planes 9 %).  That is why
+// two warpgroups take the blocks of the rows in turn (124 -> 118 us at 64 x 2048 x 128256) and each half has a warp of its own
+// that issues the multiplications, with slots and parities that are constants (one warp for both: 1450 cycles a step).  Rows
+// through registers instead of the ring took 9 % longer, a read-out two places deep as long.
+// Measured: 33 x 2048 -> 8200 10.6 us, 64 x 4096 -> 4096 16.5 us, 64 x 2048 -> 128256 118 us (mma.sync, which takes 8.5 cycles of a
+// quarter SM for 16 outputs and eight columns: 17.6, 27.4 and 426).  A launch with little to do takes 4.4 us.
 #include <cuda_runtime.h>
 
 #include <algorithm>
@@ -407,6 +414,8 @@ __global__ void __launch_bounds__(THREADS, 1) q4_rows_kernel(Q4GemvArgs a, int k
                     tmem_ld8(da + NT + c, v1);
                     tmem_ld8(da + 2 * NT + c, v2);
                     tmem_wait_ld();
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) asm volatile("" : "+r"(v0[e]), "+r"(v1[e]), "+r"(v2[e]));      // used behind the wait only
                     if (c + 8 == NT) {
                         tc_fence_before();
                         __syncwarp();
