@@ -81,6 +81,10 @@ __device__ __forceinline__ void planes(float x0, float x1, uint32_t (&p)[3]) {
     p[2] = __byte_perm(__float_as_uint(s0), __float_as_uint(s1), 0x7632);
 }
 
+// Every warp is behind this before it waits for another one: the time limit of those waits does not run while the kernel ahead in
+// the stream does.
+__device__ __forceinline__ void launched_ahead() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+
 // A place of a ring of N and the parity of its round.
 template <int N>
 struct Ring {
@@ -221,6 +225,7 @@ __global__ void __launch_bounds__(THREADS, 1) q4_rows_kernel(Q4GemvArgs a, int k
                 }
             }
         };
+        launched_ahead();
         if (warp == 0) multiply(std::integral_constant<int, 0>{});
         if (warp == 2) multiply(std::integral_constant<int, 1>{});
     } else if (wg < 3) {
@@ -263,7 +268,7 @@ __global__ void __launch_bounds__(THREADS, 1) q4_rows_kernel(Q4GemvArgs a, int k
             }
             copy_commit();
         };
-        asm volatile("griddepcontrol.wait;" ::: "memory");                     // x may come from the kernel ahead
+        launched_ahead();                                                      // x may come from the kernel ahead
         asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
 #pragma unroll 1
         for (int i = 0; i < C::NX - 1; ++i) fetch();
@@ -324,6 +329,7 @@ __global__ void __launch_bounds__(THREADS, 1) q4_rows_kernel(Q4GemvArgs a, int k
         };
 #pragma unroll 1
         for (int i = 0; i < C::NW - 1; ++i) fetch();
+        launched_ahead();
         const int rg = lane & 7, hi = (lane >> 3) & 1, turn = (rg >> 1) & 3;   // of the output that this lane unpacks
         const unsigned char* from = ring + (lane >> 4) * 512 + rg * 64;
         const uint32_t a_at = tmem + ((uint32_t)(quad * 32) << 16) + C::TMEM_A + h * C::A_SLOTS * C::A_COLS;
@@ -388,7 +394,7 @@ __global__ void __launch_bounds__(THREADS, 1) q4_rows_kernel(Q4GemvArgs a, int k
         };
 #pragma unroll 1
         for (int i = 0; i < C::NS - 1; ++i) fetch();
-        asm volatile("griddepcontrol.wait;" ::: "memory");                     // y may be read by the kernel ahead
+        launched_ahead();                                                      // y may be read by the kernel ahead
         const uint32_t d_at = tmem + ((uint32_t)(quad * 32) << 16);
         Ring<DH> rd;
         int take = 0;

@@ -1,5 +1,5 @@
 // Inline PTX of the 5th-generation tensor core path (tcgen05, tensor memory, 2-D tiled TMA without multicast,
-// pairs of CTAs) shared by the prefill attention and the Q8_0 matrix kernels, sm_100a.
+// pairs of CTAs) shared by the prefill attention and the matrix kernels of Q8_0 and 4-bit weights, sm_100a.
 #pragma once
 #include <cuda.h>
 #include "common.cuh"

@@ -157,6 +157,82 @@ def test_infinite_and_nan_activations_stay_in_their_row(ctx):
     W.close()
 
 
+@pytest.mark.parametrize("K,N,M", [(300, 40, 33), (300, 40, 64), (9000, 40, 3), (2000, 300, 10), (2000, 40000, 12)], ids=lambda v: str(v))
+def test_rows_of_one_pass_do_not_touch_each_other(ctx, K, N, M):
+    import shainet_b200 as S
+    rng = np.random.default_rng(13)
+    packed, scales = weights(rng, K, N, 64)
+    W = S.Q4Weight.from_quantized(ctx, packed, scales, K, 64)
+    x = rng.standard_normal((M, K)).astype(np.float32)
+    clean = product(ctx, W, x, N)
+    for bad in (np.nan, np.inf, -np.inf, 3e38):
+        x[1, K - 1] = bad
+        got = product(ctx, W, x, N)
+        assert np.array_equal(np.delete(got, 1, 0), np.delete(clean, 1, 0))
+        if not np.isfinite(bad):
+            assert not np.isfinite(got[1]).any()
+    W.close()
+
+
+@pytest.mark.parametrize("K,N,M", [(1, 1, 25), (31, 17, 64), (65, 15, 130), (12300, 1, 9), (127, 257, 33)], ids=lambda v: str(v))
+def test_odd_sizes_of_many_rows(ctx, K, N, M):
+    import shainet_b200 as S
+    for group in (32, 64, 128):
+        rng = np.random.default_rng(K + N + M + group)
+        packed, scales = weights(rng, K, N, group)
+        W = S.Q4Weight.from_quantized(ctx, packed, scales, K, group)
+        w, x = dense(packed, scales, K, group), rng.standard_normal((M, K)).astype(np.float32)
+        got, ref = product(ctx, W, x, N), x.astype(np.float64) @ w.T
+        assert np.abs(got - ref).max() <= tol(K) * (np.abs(x).astype(np.float64) @ np.abs(w).T).max(), rel_err(got, ref)
+        W.close()
+
+
+def test_many_rows_on_two_streams_and_in_graphs(ctx):
+    """Clusters and tensor memory under load: products of several shapes at once on two streams, then two graphs of them
+    replayed at once; every result is bit for bit that of a call by itself."""
+    import torch
+    import shainet_b200 as S
+    rng = np.random.default_rng(21)
+    made = []
+    for K, N, M, group in ((2048, 4100, 33, 128), (4096, 4096, 64, 64), (5000, 100, 40, 32), (2048, 20000, 12, 64)):
+        packed, scales = weights(rng, K, N, group)
+        W = S.Q4Weight.from_quantized(ctx, packed, scales, K, group)
+        x = torch.from_numpy(rng.standard_normal((M, K)).astype(np.float32)).cuda()
+        ys = [torch.full((M, N), float("nan"), device="cuda") for _ in range(3)]
+        torch.cuda.synchronize()
+        W.gemv_dev(x.data_ptr(), ys[0].data_ptr(), M)
+        made.append((W, x, ys, M))
+    ctx.sync()
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    for rep in range(20):
+        for i, s in enumerate(streams):
+            for W, x, ys, M in made[:: 1 - 2 * i]:
+                W.gemv_dev(x.data_ptr(), ys[1 + i].data_ptr(), M, stream=s.cuda_stream)
+    torch.cuda.synchronize()
+    ctx.sync()
+    assert all(torch.equal(ys[0], y) for _, _, ys, _ in made for y in ys[1:])
+    graphs = []
+    for i, s in enumerate(streams):
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g, stream=s):
+            for W, x, ys, M in made[:: 1 - 2 * i]:
+                W.gemv_dev(x.data_ptr(), ys[1 + i].data_ptr(), M, stream=s.cuda_stream)
+        graphs.append(g)
+    for _, _, ys, _ in made:
+        for y in ys[1:]:
+            y.fill_(float("nan"))
+    torch.cuda.synchronize()
+    for rep in range(10):
+        for g, s in zip(graphs, streams):
+            with torch.cuda.stream(s):
+                g.replay()
+    torch.cuda.synchronize()
+    ctx.sync()
+    assert all(torch.equal(ys[0], y) for _, _, ys, _ in made for y in ys[1:])
+    for W, _, _, _ in made:
+        W.close()
+
+
 @pytest.mark.parametrize("K,N,group", [(2048, 512, 32), (1001, 77, 64), (130, 3, 128)], ids=lambda v: str(v))
 def test_creation_and_export(ctx, K, N, group):
     """The three ways in hold the same weight; export gives back what went in; the quantiser follows its definition."""
