@@ -404,6 +404,16 @@ int shainet_attn_paged_plan_dev(shainet_attn_ctx* ctx, int requests, const int32
                                 int32_t* block_table, int table_width, int page_rows, int32_t* free_pages, int num_pages,
                                 const int32_t* free_count, int32_t* lens_out, int32_t* free_count_out, int32_t* first,
                                 int32_t* slots, int max_tokens, int32_t* status, void* stream);
+/* plan_dev that also writes the lengths for the decode of the same step (paged_decode_dev): decode_lens[r] = lens[r] + 1
+ * where delta[r] == 1, else 0, and 0 for every request where the step cannot be taken.  lens_out is no such list: a
+ * request that holds rows but takes no token (idle, shortened), one whose prompt of several tokens a scatter brings, and
+ * every request of a step that was refused stand there with a length above 0, and a decode over it would write the new rows
+ * over the last position that they hold.  A captured loop of plan and decode, whose status nobody reads in between, takes
+ * decode_lens.  The array overlaps no other one. */
+int shainet_attn_paged_step_dev(shainet_attn_ctx* ctx, int requests, const int32_t* lens, const int32_t* delta,
+                                int32_t* block_table, int table_width, int page_rows, int32_t* free_pages, int num_pages,
+                                const int32_t* free_count, int32_t* lens_out, int32_t* free_count_out, int32_t* first,
+                                int32_t* slots, int max_tokens, int32_t* decode_lens, int32_t* status, void* stream);
 /* The head layout and the workspace of the calls below.  Calls that use one handle run one behind another: on one
  * stream, or ordered by events or graph edges.  Streams or graphs that may run at the same time take a handle each.
  * head_dim is 64 or 128, any number of query heads per kv head. */
@@ -415,7 +425,8 @@ int shainet_attn_paged_destroy(shainet_attn_paged* paged);
  * v_new [requests, kv_dim] are raw projection outputs, out [requests, q_dim].  lens counts the new token: its position
  * is lens[r] - 1, its rotated k row and its v row are written there, and it sees the positions 0 .. lens[r] - 1.  kv is
  * the block's cache: RoPE table, norm weights, biases and head layout are its own, its rows are not touched.
- * lens[r] == 0 is a padded row: nothing is written into pages, its out row is zeros.  Lengths are read on the device, so
+ * lens[r] == 0 is a padded row: nothing is written into pages, its out row is zeros.  Every other request takes a token:
+ * behind a plan these are the decode_lens of paged_step_dev, not its lens_out.  Lengths are read on the device, so
  * the call can be captured and replayed as requests grow.  A length that the table cannot hold makes a row of zeros, a
  * table cell outside the pool is not followed (that request's out row is then unspecified); either is reported as
  * SHAINET_ATTN_E_INVALID by the next blocking call on ctx after the stream was synchronised (what the call of one request

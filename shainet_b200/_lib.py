@@ -83,6 +83,7 @@ SIGNATURES = {
     "shainet_attn_decoder_generate": (C.c_int, [_P, _P, C.POINTER(C.c_int32), C.c_int, C.c_int, C.POINTER(C.c_int32)]),
     "shainet_attn_decode_noalloc": (C.c_int, [_P, _P, _P, _P, C.c_int, C.c_int, C.c_int, C.c_int, C.c_int, C.c_float, _P]),
     "shainet_attn_paged_plan_dev": (C.c_int, [_P, C.c_int, _P, _P, _P, C.c_int, C.c_int, _P, C.c_int, _P, _P, _P, _P, _P, C.c_int, _P, _P]),
+    "shainet_attn_paged_step_dev": (C.c_int, [_P, C.c_int, _P, _P, _P, C.c_int, C.c_int, _P, C.c_int, _P, _P, _P, _P, _P, C.c_int, _P, _P, _P]),
     "shainet_attn_paged_create": (C.c_int, [_P, C.POINTER(_P), C.c_int, C.c_int, C.c_int, C.c_int, C.c_int]),
     "shainet_attn_paged_destroy": (C.c_int, [_P]),
     "shainet_attn_paged_decode_dev": (C.c_int, [_P, _P, _P, _P, _P, C.c_int, _P, _P, _P, _P, _P, C.c_int, _P, C.c_int, C.c_float, _P]),

@@ -310,9 +310,18 @@ def forward_batched_dev(ctx: AttnContext, caches, q_ptr: int, k_ptr: int, v_ptr:
 
 def plan_pages_dev(ctx: AttnContext, requests: int, lens_ptr: int, delta_ptr: int, block_table_ptr: int, table_width: int,
                    page_rows: int, free_pages_ptr: int, num_pages: int, free_count_ptr: int, lens_out_ptr: int,
-                   free_count_out_ptr: int, first_ptr: int, slots_ptr: int, max_tokens: int, status_ptr: int, stream=None):
+                   free_count_out_ptr: int, first_ptr: int, slots_ptr: int, max_tokens: int, status_ptr: int, stream=None,
+                   decode_lens_ptr: int | None = None):
     """One step of the page tables of a batch on the device: pages pushed and popped, lengths, offsets and slots of the
-    new tokens.  int32 device pointers; ``status`` receives ``_lib.PLAN_*`` and its detail."""
+    new tokens.  int32 device pointers; ``status`` receives ``_lib.PLAN_*`` and its detail.  ``decode_lens``, where given,
+    receives the lengths for ``PagedAttention.decode_dev`` of the same step: 0 for requests that take no token or a prompt,
+    and for all of a step that cannot be taken (``lens_out`` is no such list)."""
+    if decode_lens_ptr is not None:
+        check(ctx.L.shainet_attn_paged_step_dev(ctx.h, requests, lens_ptr, delta_ptr, block_table_ptr, table_width, page_rows,
+                                                free_pages_ptr, num_pages, free_count_ptr, lens_out_ptr, free_count_out_ptr,
+                                                first_ptr, slots_ptr, max_tokens, decode_lens_ptr, status_ptr,
+                                                _stream_arg(stream)))
+        return
     check(ctx.L.shainet_attn_paged_plan_dev(ctx.h, requests, lens_ptr, delta_ptr, block_table_ptr, table_width, page_rows,
                                             free_pages_ptr, num_pages, free_count_ptr, lens_out_ptr, free_count_out_ptr,
                                             first_ptr, slots_ptr, max_tokens, status_ptr, _stream_arg(stream)))
@@ -342,7 +351,8 @@ class PagedAttention:
     def decode_dev(self, attn, k_pages_ptr: int, v_pages_ptr: int, num_pages: int, q_ptr: int, k_ptr: int, v_ptr: int,
                    out_ptr: int, block_table_ptr: int, table_width: int, lens_ptr: int, requests: int, scale: float,
                    stream=None):
-        """One decode token for each request; ``lens`` counts it, 0 is a padded row."""
+        """One decode token for each request; ``lens`` counts it, 0 is a padded row (behind ``plan_pages_dev``: its
+        ``decode_lens``)."""
         check(self.L.shainet_attn_paged_decode_dev(self.ctx.h, self.h, _cache_of(attn).h, k_pages_ptr, v_pages_ptr, num_pages,
                                                    q_ptr, k_ptr, v_ptr, out_ptr, block_table_ptr, table_width, lens_ptr,
                                                    requests, scale, _stream_arg(stream)))

@@ -132,6 +132,12 @@ module SHAInet
                                                      lens_out : Int32*, free_count_out : Int32*, first : Int32*,
                                                      slots : Int32*, max_tokens : Int32, status : Int32*,
                                                      stream : Void*) : Int32
+    fun paged_step_dev = shainet_attn_paged_step_dev(ctx : Ctx, requests : Int32, lens : Int32*, delta : Int32*,
+                                                     block_table : Int32*, table_width : Int32, page_rows : Int32,
+                                                     free_pages : Int32*, num_pages : Int32, free_count : Int32*,
+                                                     lens_out : Int32*, free_count_out : Int32*, first : Int32*,
+                                                     slots : Int32*, max_tokens : Int32, decode_lens : Int32*,
+                                                     status : Int32*, stream : Void*) : Int32
     fun paged_create = shainet_attn_paged_create(ctx : Ctx, out_paged : Paged*, num_heads : Int32, num_kv_heads : Int32,
                                                  head_dim : Int32, page_rows : Int32, format : Int32) : Int32
     fun paged_destroy = shainet_attn_paged_destroy(paged : Paged) : Int32

@@ -219,7 +219,7 @@ cudaError_t launch_embed_rows(const int* ids_dev, const float* table, float* x, 
 cudaError_t launch_argmax_decode(const unsigned long long* words, int* tokens, int n, int* next_id, int* history,
                                  int history_pos, cudaStream_t s);
 
-// One step of the block tables of `requests` requests: see shainet_attn_paged_plan_dev.
+// One step of the block tables of `requests` requests: see shainet_attn_paged_plan_dev and shainet_attn_paged_step_dev.
 struct PagedPlanArgs {
     const int* lens;
     const int* delta;
@@ -230,6 +230,7 @@ struct PagedPlanArgs {
     int* free_count_out;    // may be free_count
     int* first;             // [requests + 1]
     int* slots;             // [max_tokens]
+    int* decode_lens;       // [requests], nullable
     int* status;            // [2]
     int requests, table_width, page_rows, num_pages, max_tokens;
     // set by the launch

@@ -81,14 +81,10 @@ int copy_rows(shainet_attn_ctx* ctx, const shainet_attn_paged* paged, const shai
     return SHAINET_ATTN_OK;
 }
 
-}  // namespace
-
-extern "C" {
-
-int shainet_attn_paged_plan_dev(shainet_attn_ctx* ctx, int requests, const int32_t* lens, const int32_t* delta,
-                                int32_t* block_table, int table_width, int page_rows, int32_t* free_pages, int num_pages,
-                                const int32_t* free_count, int32_t* lens_out, int32_t* free_count_out, int32_t* first,
-                                int32_t* slots, int max_tokens, int32_t* status, void* stream) {
+// decode_lens: nullable where the step is not asked for them (step_dev asks).
+int plan_step(shainet_attn_ctx* ctx, int requests, const int32_t* lens, const int32_t* delta, int32_t* block_table, int table_width,
+              int page_rows, int32_t* free_pages, int num_pages, const int32_t* free_count, int32_t* lens_out, int32_t* free_count_out,
+              int32_t* first, int32_t* slots, int max_tokens, int32_t* decode_lens, int32_t* status, void* stream) {
     if (requests < 0) return fail(SHAINET_ATTN_E_INVALID, "requests %d < 0", requests);
     if (requests > SHAINET_ATTN_PAGED_MAX_REQUESTS)
         return fail(SHAINET_ATTN_E_UNSUPPORTED, "%d requests: a step plans at most %d", requests, SHAINET_ATTN_PAGED_MAX_REQUESTS);
@@ -100,7 +96,8 @@ int shainet_attn_paged_plan_dev(shainet_attn_ctx* ctx, int requests, const int32
         (max_tokens > 0 && !slots) || !status)
         return fail(SHAINET_ATTN_E_INVALID, "null array");
     for (const void* p : {(const void*)lens, (const void*)delta, (const void*)block_table, (const void*)free_pages, (const void*)free_count,
-                          (const void*)lens_out, (const void*)free_count_out, (const void*)first, (const void*)slots, (const void*)status})
+                          (const void*)lens_out, (const void*)free_count_out, (const void*)first, (const void*)slots, (const void*)decode_lens,
+                          (const void*)status})
         if (!aligned4(p)) return fail(SHAINET_ATTN_E_INVALID, "int32 arrays must be 4-byte aligned");
     if (!ctx) return fail(SHAINET_ATTN_E_INVALID, "null context");
     DeviceGuard g(ctx->device);
@@ -114,6 +111,7 @@ int shainet_attn_paged_plan_dev(shainet_attn_ctx* ctx, int requests, const int32
     a.free_count_out = free_count_out;
     a.first = first;
     a.slots = slots;
+    a.decode_lens = decode_lens;
     a.status = status;
     a.requests = requests;
     a.table_width = table_width;
@@ -123,6 +121,28 @@ int shainet_attn_paged_plan_dev(shainet_attn_ctx* ctx, int requests, const int32
     plain_launch(ctx);
     CU(launch_paged_plan(a, stream ? (cudaStream_t)stream : ctx->stream));
     return SHAINET_ATTN_OK;
+}
+
+}  // namespace
+
+extern "C" {
+
+int shainet_attn_paged_plan_dev(shainet_attn_ctx* ctx, int requests, const int32_t* lens, const int32_t* delta,
+                                int32_t* block_table, int table_width, int page_rows, int32_t* free_pages, int num_pages,
+                                const int32_t* free_count, int32_t* lens_out, int32_t* free_count_out, int32_t* first,
+                                int32_t* slots, int max_tokens, int32_t* status, void* stream) {
+    return plan_step(ctx, requests, lens, delta, block_table, table_width, page_rows, free_pages, num_pages, free_count, lens_out,
+                     free_count_out, first, slots, max_tokens, nullptr, status, stream);
+}
+
+int shainet_attn_paged_step_dev(shainet_attn_ctx* ctx, int requests, const int32_t* lens, const int32_t* delta,
+                                int32_t* block_table, int table_width, int page_rows, int32_t* free_pages, int num_pages,
+                                const int32_t* free_count, int32_t* lens_out, int32_t* free_count_out, int32_t* first,
+                                int32_t* slots, int max_tokens, int32_t* decode_lens, int32_t* status, void* stream) {
+    if (requests > 0 && (!decode_lens || decode_lens == lens || decode_lens == lens_out))
+        return fail(SHAINET_ATTN_E_INVALID, "decode_lens is null or one of the arrays of the lengths");
+    return plan_step(ctx, requests, lens, delta, block_table, table_width, page_rows, free_pages, num_pages, free_count, lens_out,
+                     free_count_out, first, slots, max_tokens, decode_lens, status, stream);
 }
 
 int shainet_attn_paged_create(shainet_attn_ctx* ctx, shainet_attn_paged** out, int num_heads, int num_kv_heads, int head_dim,

@@ -140,6 +140,7 @@ __global__ void __launch_bounds__(PLAN_THREADS) paged_plan_kernel(PagedPlanArgs 
     for (unsigned r = t0; r < R; r += step) {
         a.lens_out[r] = s_len[r] + (ok ? s_delta[r] : 0);
         a.first[r] = ok ? s_new[r] : 0;
+        if (a.decode_lens) a.decode_lens[r] = ok && s_delta[r] == 1 ? s_len[r] + 1 : 0;
     }
     if (!ok) {
         for (unsigned t = t0; t < a.max_tokens; t += step) a.slots[t] = -1;
