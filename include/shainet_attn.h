@@ -49,7 +49,8 @@ extern "C" {
  * kernel then starts its RoPE/norm prologue and its streaming while that
  * kernel is still draining, and only waits for it before touching the scratch
  * the two share.  Without the flag nothing is assumed. */
-#define SHAINET_ATTN_F_INPUTS_READY 16u   /* ignored for the first launch after kv_truncate / kv_reset: the rows it
+#define SHAINET_ATTN_F_INPUTS_READY 16u   /* ignored for the first launch after kv_truncate / kv_reset, and for a cache's first one after
+                                             paged_gather_dev: the rows it
                                              rewrites may still be read by the launch ahead of it */
 /* Merge the split partials of the fused decode kernel with "last finisher"
  * tickets even where the flag-polling merge would be chosen (testing). */

@@ -375,10 +375,10 @@ bool single_token_rows(const shainet_attn_ctx* ctx, const HeadShape& hs, unsigne
 }
 
 // One call = `batch` sequences x T new tokens: norm/RoPE/append + attention.
-// `par` supplies the shared head shape, RoPE table, norm weights and biases.
+// `par` supplies the shared head shape, RoPE table, norm weights and biases.  `refilled`: some sequence's cache is.
 int run_step(shainet_attn_ctx* ctx, const shainet_attn_kv* par, SeqRef seqs, int batch, int T, long long total_visible,
              int max_visible, const float* q, const float* k_new, const float* v_new, float* out, float scale,
-             unsigned flags, cudaStream_t s, int pos_delta = 0, int no_append = 0, const SeqDesc* seqs_host = nullptr) {
+             unsigned flags, cudaStream_t s, bool refilled, int pos_delta = 0, int no_append = 0, const SeqDesc* seqs_host = nullptr) {
     const HeadShape hs = par->hs;
     const bool fused = T == 1 && splitk_supported(hs) && !single_token_rows(ctx, hs, flags, pos_delta, no_append) &&
                        !(flags & (SHAINET_ATTN_F_GENERIC | SHAINET_ATTN_F_UNFUSED | SHAINET_ATTN_F_TENSOR));
@@ -500,9 +500,10 @@ int run_step(shainet_attn_ctx* ctx, const shainet_attn_kv* par, SeqRef seqs, int
     }
     // A fused kernel may start while the previous fused kernel still runs; that
     // one can be appending the newest row of this very cache.
-    f.unsafe_tail = (ctx->last_fused || ctx->after_chain_kernel) ? 1 : 0;
+    // A copy out of pages promises its rows only to what has waited for it: none is fetched ahead of the wait.
+    f.unsafe_tail = refilled ? ALL_ROWS : (ctx->last_fused || ctx->after_chain_kernel) ? 1 : 0;
     ctx->after_chain_kernel = false;
-    f.inputs_ready = ((flags & SHAINET_ATTN_F_INPUTS_READY) && !ctx->rows_rewound) ? 1 : 0;
+    f.inputs_ready = ((flags & SHAINET_ATTN_F_INPUTS_READY) && !ctx->rows_rewound && !refilled) ? 1 : 0;
     ctx->rows_rewound = false;
     f.pos_delta = pos_delta;
     f.no_append = no_append;
@@ -589,8 +590,9 @@ int forward_device(shainet_attn_ctx* ctx, shainet_attn_kv* kv, const float* q, c
     seqs.one = SeqDesc{kv->k, kv->v, kv->len, kv->cap};
     seqs.many = nullptr;
     const long long total_visible = (long long)T * kv->len + (long long)T * (T + 1) / 2;
-    rc = run_step(ctx, kv, seqs, 1, T, total_visible, kv->len + T, q, k_new, v_new, out, scale, flags, s);
+    rc = run_step(ctx, kv, seqs, 1, T, total_visible, kv->len + T, q, k_new, v_new, out, scale, flags, s, kv->refilled);
     if (rc) return rc;
+    kv->refilled = false;
     kv->len += T;
     return SHAINET_ATTN_OK;
 }
@@ -1085,8 +1087,9 @@ int shainet_attn_forward_dev_at(shainet_attn_ctx* ctx, shainet_attn_kv* kv, cons
     seqs.one = SeqDesc{kv->k, kv->v, kv->len, kv->cap};
     seqs.many = nullptr;
     const int visible = kv->len + (append ? 1 : 0);
-    rc = run_step(ctx, kv, seqs, 1, 1, visible, visible, q, k_new, v_new, out, scale, flags, s, position - kv->len, append ? 0 : 1);
+    rc = run_step(ctx, kv, seqs, 1, 1, visible, visible, q, k_new, v_new, out, scale, flags, s, kv->refilled, position - kv->len, append ? 0 : 1);
     if (rc) return rc;
+    kv->refilled = false;
     if (append) kv->len += 1;
     return SHAINET_ATTN_OK;
 }
@@ -1285,7 +1288,9 @@ int shainet_attn_forward_batched_dev(shainet_attn_ctx* ctx, shainet_attn_kv* con
     SeqDesc* dd = ctx->seq_dev + (size_t)slot * ctx->seq_cap;
     long long total_visible = 0;
     int max_visible = 0;
+    bool refilled = false;
     for (int b = 0; b < batch; ++b) {
+        refilled |= kvs[b]->refilled;
         hd[b] = SeqDesc{kvs[b]->k, kvs[b]->v, kvs[b]->len, kvs[b]->cap};
         total_visible += kvs[b]->len + 1;
         max_visible = std::max(max_visible, kvs[b]->len + 1);
@@ -1294,9 +1299,12 @@ int shainet_attn_forward_batched_dev(shainet_attn_ctx* ctx, shainet_attn_kv* con
     CU(cudaEventRecord(ctx->seq_ev[slot], s));
     SeqRef seqs{};
     seqs.many = dd;
-    rc = run_step(ctx, first, seqs, batch, 1, total_visible, max_visible, q, k_new, v_new, out, scale, flags, s, 0, 0, hd);
+    rc = run_step(ctx, first, seqs, batch, 1, total_visible, max_visible, q, k_new, v_new, out, scale, flags, s, refilled, 0, 0, hd);
     if (rc) return rc;
-    for (int b = 0; b < batch; ++b) kvs[b]->len += 1;
+    for (int b = 0; b < batch; ++b) {
+        kvs[b]->refilled = false;
+        kvs[b]->len += 1;
+    }
     return SHAINET_ATTN_OK;
 }
 

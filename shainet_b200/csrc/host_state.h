@@ -91,6 +91,8 @@ struct shainet_attn_kv {
     std::vector<Mapping> mappings;
     int cap = 0;
     int len = 0;
+    bool refilled = false;      // a copy out of pages has written rows since the last launch on this cache and may still run: the
+                                // next launch reads no row, and takes no input for granted, ahead of its wait for it
     float* inv_freq = nullptr;  // device, head_dim/2
     float* q_norm = nullptr;    // device, nullable
     float* k_norm = nullptr;

@@ -57,7 +57,8 @@ int check_paged(shainet_attn_ctx* ctx, const shainet_attn_paged* paged, const sh
 }
 
 // A paged call's kernel touches nothing before all work ahead of it in the stream is complete, and lets the next kernel
-// launch only then or at its end: a fused decode kernel behind it finds no row of a contiguous cache under construction.
+// launch only then or at its end: a fused decode kernel behind it finds no row under construction by a launch before it.
+// (What the kernel itself has written, the rows of a gather, counts for the next one only behind that one's own wait.)
 void plain_launch(shainet_attn_ctx* ctx) { ctx->last_fused = false; }
 
 int copy_rows(shainet_attn_ctx* ctx, const shainet_attn_paged* paged, const shainet_attn_kv* kv, void* k_pages, void* v_pages,
@@ -266,7 +267,7 @@ int shainet_attn_paged_gather_dev(shainet_attn_ctx* ctx, shainet_attn_paged* pag
             rc = copy_rows(ctx, paged, kv, const_cast<void*>(k_pages), const_cast<void*>(v_pages), num_pages, table_row, 0, rows, false, s);
         if (rc) return rc;
     }
-    ctx->rows_rewound = true;   // the rows are others than the launch ahead may still read
+    kv->refilled = true;
     kv->len = rows;
     return SHAINET_ATTN_OK;
 }

@@ -20,7 +20,8 @@ __global__ void __launch_bounds__(COPY_THREADS) paged_copy_kernel(PagedCopyArgs 
     constexpr int STEP = COPY_THREADS / CHUNKS;
     const int piece = threadIdx.x % CHUNKS, h = blockIdx.y;
     const int i0 = blockIdx.x * (STEP * COPY_ROWS) + threadIdx.x / CHUNKS;
-    // The next kernel in the stream is not let in before this one's end: it may read rows of a cache ahead of its own wait.
+    // The next kernel in the stream is not let in before this one's last stores have been issued; that they can be seen is
+    // promised to its own wait alone, so the launch behind a gather reads no row of that cache ahead of it.
     asm volatile("griddepcontrol.wait;" ::: "memory");
     size_t at_page[COPY_ROWS];
     bool on[COPY_ROWS];
