@@ -16,6 +16,9 @@
  * only the context's own stream: a caller that launched on a stream of its own
  * synchronises that stream first (ctx_sync also reports a kernel-side wait failure
  * only once the stream that ran the kernel has been synchronised).
+ * The attention calls of a context (forward_*, the block and decoder entries) share its scratch: calls on different
+ * streams that could run at the same time are ordered by the caller, or use a context each.  Paged calls and products
+ * with 4-bit weights use none of it; what they share is said with them.
  * There is no CPU fallback: without a CUDA device every call fails.
  */
 #ifndef SHAINET_ATTN_H
@@ -49,9 +52,9 @@ extern "C" {
  * kernel then starts its RoPE/norm prologue and its streaming while that
  * kernel is still draining, and only waits for it before touching the scratch
  * the two share.  Without the flag nothing is assumed. */
-#define SHAINET_ATTN_F_INPUTS_READY 16u   /* ignored for the first launch after kv_truncate / kv_reset, and for a cache's first one after
-                                             paged_gather_dev: the rows it
-                                             rewrites may still be read by the launch ahead of it */
+#define SHAINET_ATTN_F_INPUTS_READY 16u   /* ignored for a cache's first launch after kv_truncate, kv_reset or paged_gather_dev:
+                                             the launch ahead of it may still read the rows it rewrites, or write
+                                             the rows it reads */
 /* Merge the split partials of the fused decode kernel with "last finisher"
  * tickets even where the flag-polling merge would be chosen (testing). */
 #define SHAINET_ATTN_F_TICKET_MERGE 32u

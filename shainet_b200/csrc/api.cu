@@ -374,11 +374,19 @@ bool single_token_rows(const shainet_attn_ctx* ctx, const HeadShape& hs, unsigne
            !(flags & (SHAINET_ATTN_F_SPLITK | SHAINET_ATTN_F_TICKET_MERGE));
 }
 
+// What a launch on some caches has to know of the ones ahead of it (shainet_attn_kv).
+struct Ahead {
+    bool rewound = false, refilled = false;
+};
+Ahead ahead_of(const shainet_attn_kv* kv) { return Ahead{kv->rewound, kv->refilled}; }
+// Every launch waits for what was enqueued before it in its stream, and lets its successor in only then.
+void launched(shainet_attn_kv* kv) { kv->rewound = kv->refilled = false; }
+
 // One call = `batch` sequences x T new tokens: norm/RoPE/append + attention.
-// `par` supplies the shared head shape, RoPE table, norm weights and biases.  `refilled`: some sequence's cache is.
+// `par` supplies the shared head shape, RoPE table, norm weights and biases.
 int run_step(shainet_attn_ctx* ctx, const shainet_attn_kv* par, SeqRef seqs, int batch, int T, long long total_visible,
              int max_visible, const float* q, const float* k_new, const float* v_new, float* out, float scale,
-             unsigned flags, cudaStream_t s, bool refilled, int pos_delta = 0, int no_append = 0, const SeqDesc* seqs_host = nullptr) {
+             unsigned flags, cudaStream_t s, Ahead ahead, int pos_delta = 0, int no_append = 0, const SeqDesc* seqs_host = nullptr) {
     const HeadShape hs = par->hs;
     const bool fused = T == 1 && splitk_supported(hs) && !single_token_rows(ctx, hs, flags, pos_delta, no_append) &&
                        !(flags & (SHAINET_ATTN_F_GENERIC | SHAINET_ATTN_F_UNFUSED | SHAINET_ATTN_F_TENSOR));
@@ -397,7 +405,6 @@ int run_step(shainet_attn_ctx* ctx, const shainet_attn_kv* par, SeqRef seqs, int
     if (!fused && kern != Kernel::Rows && par->es != 4 && seqs.many != nullptr)
         return fail(SHAINET_ATTN_E_UNSUPPORTED, "batched decode over bfloat16 caches is not served by a forced kernel");
     if (!fused) {
-        ctx->last_fused = false;
         rc = grow(ctx->q_rot, (size_t)batch * T * hs.num_heads * hs.head_dim, s);
         if (rc) return rc;
         PrepArgs p{};
@@ -498,13 +505,12 @@ int run_step(shainet_attn_ctx* ctx, const shainet_attn_kv* par, SeqRef seqs, int
         }
         f.epoch = ++ctx->epoch;
     }
-    // A fused kernel may start while the previous fused kernel still runs; that
-    // one can be appending the newest row of this very cache.
+    // A fused kernel may start while an earlier launch in its stream still runs, which can be the fused kernel that appends
+    // the newest row of this very cache: directly ahead of it, or behind kernels that let their successor in early.  What else
+    // was called on this context, on whichever stream, says nothing about that row, so it is never fetched ahead of the wait.
     // A copy out of pages promises its rows only to what has waited for it: none is fetched ahead of the wait.
-    f.unsafe_tail = refilled ? ALL_ROWS : (ctx->last_fused || ctx->after_chain_kernel) ? 1 : 0;
-    ctx->after_chain_kernel = false;
-    f.inputs_ready = ((flags & SHAINET_ATTN_F_INPUTS_READY) && !ctx->rows_rewound && !refilled) ? 1 : 0;
-    ctx->rows_rewound = false;
+    f.unsafe_tail = ahead.refilled ? ALL_ROWS : 1;
+    f.inputs_ready = ((flags & SHAINET_ATTN_F_INPUTS_READY) && !ahead.rewound && !ahead.refilled) ? 1 : 0;
     f.pos_delta = pos_delta;
     f.no_append = no_append;
     f.kv_elem_bytes = par->es;
@@ -541,7 +547,6 @@ int run_step(shainet_attn_ctx* ctx, const shainet_attn_kv* par, SeqRef seqs, int
         CU(cudaEventRecord(ev.second, s));
         ctx->timed.push_back(ev);
     }
-    ctx->last_fused = true;
     return SHAINET_ATTN_OK;
 }
 
@@ -582,17 +587,15 @@ bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) ==
 
 int forward_device(shainet_attn_ctx* ctx, shainet_attn_kv* kv, const float* q, const float* k_new, const float* v_new,
                    float* out, int T, float scale, unsigned flags, cudaStream_t s) {
-    const int cap_before = kv->cap;
     int rc = kv_ensure(kv, kv->len + T, s);
     if (rc) return rc;
-    if (kv->cap != cap_before) ctx->last_fused = false;  // growth synchronised the stream
     SeqRef seqs{};
     seqs.one = SeqDesc{kv->k, kv->v, kv->len, kv->cap};
     seqs.many = nullptr;
     const long long total_visible = (long long)T * kv->len + (long long)T * (T + 1) / 2;
-    rc = run_step(ctx, kv, seqs, 1, T, total_visible, kv->len + T, q, k_new, v_new, out, scale, flags, s, kv->refilled);
+    rc = run_step(ctx, kv, seqs, 1, T, total_visible, kv->len + T, q, k_new, v_new, out, scale, flags, s, ahead_of(kv));
     if (rc) return rc;
-    kv->refilled = false;
+    launched(kv);
     kv->len += T;
     return SHAINET_ATTN_OK;
 }
@@ -833,14 +836,14 @@ int shainet_attn_kv_destroy(shainet_attn_kv* kv) {
 int shainet_attn_kv_reset(shainet_attn_kv* kv) {
     if (!kv) return fail(SHAINET_ATTN_E_INVALID, "null cache");
     kv->len = 0;  // buffers stay; stale rows are rewritten before they become visible
-    kv->ctx->rows_rewound = true;
+    kv->rewound = true;
     return SHAINET_ATTN_OK;
 }
 
 int shainet_attn_kv_truncate(shainet_attn_kv* kv, int len) {
     if (!kv) return fail(SHAINET_ATTN_E_INVALID, "null cache");
     if (len < 0 || len > kv->len) return fail(SHAINET_ATTN_E_STATE, "truncate to %d of a cache of %d", len, kv->len);
-    if (len < kv->len) kv->ctx->rows_rewound = true;
+    if (len < kv->len) kv->rewound = true;
     kv->len = len;
     return SHAINET_ATTN_OK;
 }
@@ -1079,17 +1082,15 @@ int shainet_attn_forward_dev_at(shainet_attn_ctx* ctx, shainet_attn_kv* kv, cons
     if (!append && kv->len == 0) return fail(SHAINET_ATTN_E_STATE, "nothing to attend to: the cache is empty and the token is not appended");
     DeviceGuard g(ctx->device);
     cudaStream_t s = stream ? (cudaStream_t)stream : ctx->stream;
-    const int cap_before = kv->cap;
     rc = kv_ensure(kv, kv->len + (append ? 1 : 0), s);
     if (rc) return rc;
-    if (kv->cap != cap_before) ctx->last_fused = false;
     SeqRef seqs{};
     seqs.one = SeqDesc{kv->k, kv->v, kv->len, kv->cap};
     seqs.many = nullptr;
     const int visible = kv->len + (append ? 1 : 0);
-    rc = run_step(ctx, kv, seqs, 1, 1, visible, visible, q, k_new, v_new, out, scale, flags, s, kv->refilled, position - kv->len, append ? 0 : 1);
+    rc = run_step(ctx, kv, seqs, 1, 1, visible, visible, q, k_new, v_new, out, scale, flags, s, ahead_of(kv), position - kv->len, append ? 0 : 1);
     if (rc) return rc;
-    kv->refilled = false;
+    launched(kv);
     if (append) kv->len += 1;
     return SHAINET_ATTN_OK;
 }
@@ -1101,7 +1102,6 @@ int shainet_attn_merge_parts(shainet_attn_ctx* ctx, const float* gathered_dev, i
         return fail(SHAINET_ATTN_E_INVALID, "bad partition: %d ranks in groups of %d", world, seq_parts);
     DeviceGuard g(ctx->device);
     cudaStream_t s = stream ? (cudaStream_t)stream : ctx->stream;
-    ctx->last_fused = false;
     CU(launch_merge_parts(gathered_dev, world, seq_parts, heads_per_rank, head_dim, out_full_dev, s));
     return SHAINET_ATTN_OK;
 }
@@ -1288,9 +1288,10 @@ int shainet_attn_forward_batched_dev(shainet_attn_ctx* ctx, shainet_attn_kv* con
     SeqDesc* dd = ctx->seq_dev + (size_t)slot * ctx->seq_cap;
     long long total_visible = 0;
     int max_visible = 0;
-    bool refilled = false;
+    Ahead ahead;
     for (int b = 0; b < batch; ++b) {
-        refilled |= kvs[b]->refilled;
+        ahead.rewound |= kvs[b]->rewound;
+        ahead.refilled |= kvs[b]->refilled;
         hd[b] = SeqDesc{kvs[b]->k, kvs[b]->v, kvs[b]->len, kvs[b]->cap};
         total_visible += kvs[b]->len + 1;
         max_visible = std::max(max_visible, kvs[b]->len + 1);
@@ -1299,10 +1300,10 @@ int shainet_attn_forward_batched_dev(shainet_attn_ctx* ctx, shainet_attn_kv* con
     CU(cudaEventRecord(ctx->seq_ev[slot], s));
     SeqRef seqs{};
     seqs.many = dd;
-    rc = run_step(ctx, first, seqs, batch, 1, total_visible, max_visible, q, k_new, v_new, out, scale, flags, s, refilled, 0, 0, hd);
+    rc = run_step(ctx, first, seqs, batch, 1, total_visible, max_visible, q, k_new, v_new, out, scale, flags, s, ahead, 0, 0, hd);
     if (rc) return rc;
     for (int b = 0; b < batch; ++b) {
-        kvs[b]->refilled = false;
+        launched(kvs[b]);
         kvs[b]->len += 1;
     }
     return SHAINET_ATTN_OK;

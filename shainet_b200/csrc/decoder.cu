@@ -136,8 +136,6 @@ int gemv(shainet_attn_ctx* ctx, const float* x, const signed char* q, const floa
     a.K = K;
     if ((size_t)K * sizeof(float) > 200 * 1024) return fail(SHAINET_ATTN_E_UNSUPPORTED, "input width %d exceeds what one CTA stages in shared memory", K);
     CU(launch_q8_gemv(a, ctx->sm_count, s));
-    ctx->last_fused = false;
-    ctx->after_chain_kernel = true;
     return SHAINET_ATTN_OK;
 }
 
@@ -169,8 +167,6 @@ int gemm_tc(shainet_attn_ctx* ctx, const Q8Maps* w0, const Q8Maps* w1, int M, in
     CU(launch_q8_gemm_tc(g, plan, ctx->sm_count, s));
     if (defer) *defer = plan.splits;
     else if (plan.splits > 1) CU(launch_q8_reduce(ctx->gemm_part.p, plan.splits, stride, M, N, out, s));
-    ctx->last_fused = false;
-    ctx->after_chain_kernel = true;
     return SHAINET_ATTN_OK;
 }
 

@@ -52,12 +52,6 @@ struct shainet_attn_ctx {
     unsigned* tickets = nullptr;        // split-merge tickets of the fused decode kernel, zero between launches
     size_t tickets_cap = 0;
     unsigned epoch = 0;                 // tag of the newest word-merged decode launch
-    bool last_fused = false;            // the newest launch on this context was a fused decode kernel
-    bool after_chain_kernel = false;    // the newest launch was a kernel of the decoder chain (programmatic launch): a fused
-                                        // decode kernel behind it may become resident while the chain's previous attention
-                                        // kernel still appends its row
-    bool rows_rewound = false;          // a cache was truncated or reset since: the next launch may rewrite rows the
-                                        // previous one still reads, so it must not run ahead of it (F_INPUTS_READY is ignored once)
     unsigned long long peer_wait_ns = shainet::WAIT_LIMIT_NS;   // limit of the waits for other ranks' exchange words
     float* lse_out = nullptr;           // caller-owned device buffer for log-sum-exp values (nullable)
     // exchange buffer shared with the other ranks of the box (IPC): comm_data_floats
@@ -91,6 +85,8 @@ struct shainet_attn_kv {
     std::vector<Mapping> mappings;
     int cap = 0;
     int len = 0;
+    bool rewound = false;       // truncated or reset since the last launch on this cache: the next one may rewrite rows that the
+                                // launch ahead still reads, so it must not run ahead of it (F_INPUTS_READY is ignored once)
     bool refilled = false;      // a copy out of pages has written rows since the last launch on this cache and may still run: the
                                 // next launch reads no row, and takes no input for granted, ahead of its wait for it
     float* inv_freq = nullptr;  // device, head_dim/2

@@ -114,7 +114,7 @@ struct FusedArgs {
     unsigned epoch;        // this launch's tag in the {value, epoch} partial words: never 0, never reused while old words exist
     int stream_merge;      // partials travel as {value, epoch} words and are folded by CTAs that poll them (single
                            // sequence, grid fully resident); part_o / part_ml then point at 8-byte words, not floats
-    int unsafe_tail;       // newest cache rows a still-running previous grid may be writing; ALL_ROWS where it may be any of them
+    int unsafe_tail;       // newest cache rows a still-running grid ahead may be writing, at least 1; ALL_ROWS where it may be any of them
     int inputs_ready;      // caller vouches that q/k_new/v_new do not come from the previous grid
     int pos_delta;         // RoPE position of the new token minus the rows already cached (0 unless the sequence is split over ranks)
     int no_append;         // attend over the cached rows only: k_new/v_new are not used, nothing is appended

@@ -57,10 +57,8 @@ int check_paged(shainet_attn_ctx* ctx, const shainet_attn_paged* paged, const sh
 }
 
 // A paged call's kernel touches nothing before all work ahead of it in the stream is complete, and lets the next kernel
-// launch only then or at its end: a fused decode kernel behind it finds no row under construction by a launch before it.
-// (What the kernel itself has written, the rows of a gather, counts for the next one only behind that one's own wait.)
-void plain_launch(shainet_attn_ctx* ctx) { ctx->last_fused = false; }
-
+// launch only then or at its end.  (What the kernel itself has written, the rows of a gather, counts for the next one only
+// behind that one's own wait.)
 int copy_rows(shainet_attn_ctx* ctx, const shainet_attn_paged* paged, const shainet_attn_kv* kv, void* k_pages, void* v_pages,
               int num_pages, const int32_t* index, int row0, int rows, bool scatter, cudaStream_t s) {
     PagedCopyArgs a{};
@@ -77,7 +75,6 @@ int copy_rows(shainet_attn_ctx* ctx, const shainet_attn_paged* paged, const shai
     a.rows = rows;
     a.row_bytes = paged->hs.head_dim * paged->es;
     a.status = ctx->status_dev;
-    plain_launch(ctx);
     CU(launch_paged_copy(a, scatter, s));
     return SHAINET_ATTN_OK;
 }
@@ -119,7 +116,6 @@ int plan_step(shainet_attn_ctx* ctx, int requests, const int32_t* lens, const in
     a.page_rows = page_rows;
     a.num_pages = num_pages;
     a.max_tokens = max_tokens;
-    plain_launch(ctx);
     CU(launch_paged_plan(a, stream ? (cudaStream_t)stream : ctx->stream));
     return SHAINET_ATTN_OK;
 }
@@ -228,7 +224,6 @@ int shainet_attn_paged_decode_dev(shainet_attn_ctx* ctx, shainet_attn_paged* pag
     a.scale = scale;
     a.kv_elem_bytes = paged->es;
     a.status = ctx->status_dev;
-    plain_launch(ctx);
     CU(launch_paged_decode(a, paged->plan, paged->workspace, paged->counters, stream ? (cudaStream_t)stream : ctx->stream));
     return SHAINET_ATTN_OK;
 }

@@ -629,7 +629,6 @@ int shainet_attn_q4_gemv_dev(shainet_attn_ctx* ctx, const shainet_attn_q4* w, co
     a.K = w->K;
     a.group = w->group;
     a.status = ctx->status_dev;
-    ctx->last_fused = false;
     CU(launch_q4_gemv(a, ctx->sm_count, stream ? (cudaStream_t)stream : ctx->stream));
     return SHAINET_ATTN_OK;
 }

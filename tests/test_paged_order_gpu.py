@@ -1,5 +1,6 @@
 """Order of calls on one stream and on several: a decode token straight behind the copy that filled its cache from pages.  The
-launch may start while the copy ends; it must see every row of it.  Outputs are compared bit for bit with the same calls
+launch may start while the copy ends; it must see every row of it.  And decode tokens of one sequence with calls of the same
+context on another stream in between, which say nothing about the row that the token before still appends.  Outputs are compared bit for bit with the same calls
 that wait for each other on the host."""
 import numpy as np
 import pytest
@@ -156,3 +157,66 @@ def test_an_emptied_cache_starts_again(ctx):
     t.wait()
     assert t.torch.equal(out, ref) and len(t.attn.cache) == 1
     t.close()
+
+
+@pytest.mark.parametrize("kv", ["f32", "bf16"])
+@pytest.mark.parametrize("between", ["q4", "q4_rows", "plan", "paged_decode"])
+def test_tokens_of_one_sequence_with_calls_on_another_stream_between(ctx, between, kv):
+    """Token, a call elsewhere, token, ...: every token sees the row of the one before it.  The rows are large against what
+    else the sequence holds, so that a row read too early (what an earlier round left there, times minus one) shows."""
+    import torch
+    import shainet_b200 as S
+    sh, n, steps = SHAPES["L1B"], 37, 60
+    H, KV, hd = sh["H"], sh["KV"], sh["hd"]
+    attn = S.LlamaAttention(ctx, H, KV, hd, sh["theta"], kv_format=kv, initial_capacity=512)
+    side = S.LlamaAttention(ctx, H, KV, hd, sh["theta"], kv_format=kv)      # gives the paged decode its parameters
+    paged = S.PagedAttention(ctx, H, KV, hd, 16, kv)
+    rng = np.random.default_rng(4)
+    W = S.Q4Weight.from_simple(ctx, rng.standard_normal((256, 512)).astype(np.float32), 64)
+    gen = torch.Generator("cuda").manual_seed(5)
+    r = lambda *s: torch.randn(*s, generator=gen, device="cuda")
+    x, y = r(40, 256), torch.empty(40, 512, device="cuda")
+    ints = lambda *v: torch.tensor(v, dtype=torch.int32, device="cuda")
+    lens, delta, table, free, count = ints(5), ints(1), ints(0, 1, -1), ints(2, 3, -1, -1), ints(2)
+    lo, co, first, slots, status = ints(0), ints(0), ints(0, 0), ints(0, 0, 0, 0), ints(0, 0)
+    dt = torch.float32 if kv == "f32" else torch.bfloat16
+    kp, vp = r(4, KV, 16, hd).to(dt), r(4, KV, 16, hd).to(dt)
+    sq, sk, sv, so = r(H * hd), r(KV * hd), r(KV * hd), torch.empty(H * hd, device="cuda")
+    q, k, v = r(steps, H * hd), r(steps, KV * hd), 3.0 * r(steps, KV * hd)
+    a, b = torch.cuda.Stream(), torch.cuda.Stream()
+
+    def elsewhere():
+        s = b.cuda_stream
+        if between in ("q4", "q4_rows"):
+            W.gemv_dev(x.data_ptr(), y.data_ptr(), 1 if between == "q4" else 40, stream=s)
+        if between == "plan":
+            S.plan_pages_dev(ctx, 1, lens.data_ptr(), delta.data_ptr(), table.data_ptr(), 3, 16, free.data_ptr(), 4, count.data_ptr(),
+                             lo.data_ptr(), co.data_ptr(), first.data_ptr(), slots.data_ptr(), 4, status.data_ptr(), stream=s)
+        if between == "paged_decode":
+            paged.decode_dev(side, kp.data_ptr(), vp.data_ptr(), 4, sq.data_ptr(), sk.data_ptr(), sv.data_ptr(), so.data_ptr(),
+                             table.data_ptr(), 3, lens.data_ptr(), 1, 0.125, stream=s)
+
+    def round_(sign, wait, flags=0):
+        attn.clear_cache()
+        attn.cache.fill_normal(n, 6)
+        vs = (sign * v).contiguous()
+        out = torch.full((steps, H * hd), float("nan"), device="cuda")
+        torch.cuda.synchronize()
+        for i in range(steps):
+            attn.forward_cached_dev(q[i].data_ptr(), k[i].data_ptr(), vs[i].data_ptr(), out[i].data_ptr(), 1, stream=a.cuda_stream,
+                                    flags=flags)
+            if wait:
+                torch.cuda.synchronize()
+            else:
+                elsewhere()
+        torch.cuda.synchronize()
+        ctx.sync()
+        return out
+
+    want = {s: round_(s, True) for s in (1.0, -1.0)}
+    for rep in range(8):
+        for s in (1.0, -1.0):
+            assert torch.equal(round_(s, False), want[s]), (rep, s)
+            assert torch.equal(round_(s, False, S.F_INPUTS_READY), want[s]), (rep, s)
+    for o in (W, paged, side, attn):
+        o.close()
