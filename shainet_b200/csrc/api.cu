@@ -189,13 +189,16 @@ int kv_ensure(shainet_attn_kv* kv, int total_len, cudaStream_t s) {
 
 int check_status(shainet_attn_ctx* ctx) {
     if (ctx->status_host && ctx->status_host->code != DEV_OK) {
-        const int code = ctx->status_host->code, where = ctx->status_host->where;
+        const int where = ctx->status_host->where;
         ctx->status_host->code = DEV_OK;
         ctx->status_host->where = 0;
-        if (code == DEV_BAD_PAGE)
-            return fail(SHAINET_ATTN_E_INVALID, "a paged call met a table cell or slot outside its pool, or a length outside its table (site %d)", where);
         if (ctx->tickets) cudaMemset(ctx->tickets, 0, ctx->tickets_cap * sizeof(unsigned));  // an unwound kernel may leave counts
         return fail(SHAINET_ATTN_E_DEVICE_WAIT, "a kernel gave up on a bounded wait (site %d)", where);
+    }
+    if (ctx->status_host && ctx->status_host->bad_page != 0) {
+        const int where = ctx->status_host->bad_page;
+        ctx->status_host->bad_page = 0;
+        return fail(SHAINET_ATTN_E_INVALID, "a paged call met a table cell or slot outside its pool, or a length outside its table (site %d)", where);
     }
     return SHAINET_ATTN_OK;
 }
@@ -638,6 +641,7 @@ int shainet_attn_ctx_create(shainet_attn_ctx** out, int device) {
     if (e == cudaSuccess) {
         c->status_host->code = DEV_OK;
         c->status_host->where = 0;
+        c->status_host->bad_page = 0;
         e = cudaHostGetDevicePointer(&c->status_dev, c->status_host, 0);
     }
     for (int i = 0; i < SEQ_RING && e == cudaSuccess; ++i) e = cudaEventCreateWithFlags(&c->seq_ev[i], cudaEventDisableTiming);

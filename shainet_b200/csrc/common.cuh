@@ -14,12 +14,14 @@ namespace shainet {
 enum DeviceStatus : int {
     DEV_OK = 0,
     DEV_WAIT_TIMEOUT = 1,   // an mbarrier wait ran past its time limit
-    DEV_BAD_PAGE = 2,       // a table cell, slot or length outside the pool or its table
 };
 
 struct AttnStatus {
     int code;
     int where;   // kernel-specific location id of the first failure
+    // A table cell, slot or length outside the pool or its table: the location id of the first one, 0 for none.  A word of its
+    // own, so that neither kind of failure hides the other.
+    int bad_page;
 };
 
 // ~1 s at the nominal 1 GHz global timer; long enough that only a programming
@@ -96,9 +98,9 @@ __device__ __forceinline__ void bulk_g2s(void* smem_dst, const void* gsrc, uint3
         : "memory");
 }
 
-// Records the first failure of a context for its next blocking call; the kernel carries on without the bad access.
-__device__ __forceinline__ void report_status(AttnStatus* status, int code, int where) {
-    if (status != nullptr && atomicCAS(&status->code, DEV_OK, code) == DEV_OK) status->where = where;
+// Records a context's first bad page for its next blocking call; the kernel carries on without the access.
+__device__ __forceinline__ void report_bad_page(AttnStatus* status, int where) {
+    if (status != nullptr) atomicCAS(&status->bad_page, 0, where);
 }
 
 __device__ __forceinline__ float4 lds128(const float* p) { return *reinterpret_cast<const float4*>(p); }

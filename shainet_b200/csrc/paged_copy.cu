@@ -31,14 +31,14 @@ __global__ void __launch_bounds__(COPY_THREADS) paged_copy_kernel(PagedCopyArgs 
         on[k] = i < a.rows;
         if (SCATTER) {
             const int slot = on[k] ? a.index[i] : -1;
-            if (slot >= 0 && !slot_in_pool(slot, a.num_pages, a.page_rows)) report_status(a.status, DEV_BAD_PAGE, 11);
+            if (slot >= 0 && !slot_in_pool(slot, a.num_pages, a.page_rows)) report_bad_page(a.status, 11);
             on[k] = slot_in_pool(slot, a.num_pages, a.page_rows);
             const int page = divide(on[k] ? slot : 0, a.by_page);
             at_page[k] = pool_row(page, a.num_kv_heads, h, a.page_rows, (on[k] ? slot : 0) - page * a.page_rows) * CHUNKS + piece;
         } else {
             const int col = divide(on[k] ? i : 0, a.by_page), page = a.index[col];
             if (on[k] && !page_in_pool(page, a.num_pages)) {
-                report_status(a.status, DEV_BAD_PAGE, 12);
+                report_bad_page(a.status, 12);
                 on[k] = false;
             }
             at_page[k] = pool_row(on[k] ? page : 0, a.num_kv_heads, h, a.page_rows, (on[k] ? i : 0) - (on[k] ? col * a.page_rows : 0)) * CHUNKS + piece;

@@ -195,7 +195,7 @@ __device__ __forceinline__ Place lookup_page(const PagedDecodeArgs& a, const Cur
 __device__ __forceinline__ unsigned row_of(const PagedDecodeArgs& a, int kv_h, Place p) {
     if (p.row < 0) return 0u;
     if (!page_in_pool(p.page, a.num_pages)) {
-        report_status(a.status, DEV_BAD_PAGE, 14);
+        report_bad_page(a.status, 14);
         return 0u;
     }
     return ((unsigned)p.page * a.hs.num_kv_heads + kv_h) * a.page_rows + p.row;
@@ -568,7 +568,7 @@ __device__ __forceinline__ void prepare_rows(const PagedDecodeArgs& a, const Seg
         const int col = divide(pos, a.by_page), page = a.block_table[(size_t)s.b * a.table_width + col];
         stores = page_in_pool(page, a.num_pages);
         if (stores) at = pool_row(page, a.hs.num_kv_heads, s.kv_h, a.page_rows, pos - col * a.page_rows) * HD;
-        else if (warp == 0 && lane == 0) report_status(a.status, DEV_BAD_PAGE, 15);
+        else if (warp == 0 && lane == 0) report_bad_page(a.status, 15);
     }
 #pragma unroll 1
     for (int it = warp; it < items; it += NW) {      // the rows this warp requested
@@ -854,7 +854,7 @@ __global__ void __launch_bounds__(THREADS, CTAS_PER_SM) paged_decode_kernel(Page
     for (int b = cta; b < a.requests; b += gridDim.x) {
         const int len = a.lens[b];
         if (valid_len(len, a.max_len) > 0 && !too_long) continue;
-        if (len != 0 && tid == 0) report_status(a.status, DEV_BAD_PAGE, 13);
+        if (len != 0 && tid == 0) report_bad_page(a.status, 13);
 #pragma unroll 1
         for (int d = tid; d < H * HD / 4; d += THREADS) reinterpret_cast<float4*>(a.out)[(size_t)b * (H * HD / 4) + d] = make_float4(0.f, 0.f, 0.f, 0.f);
     }
