@@ -402,6 +402,12 @@ __global__ void __launch_bounds__(THREADS, C::MT == 0 ? (C::NT == 1 ? 3 : 2) : 1
 
 size_t plane_bytes(const Q4GemvArgs& a) { return (size_t)blocks_of(a.K, 64) * 2 * 3 * a.M * 64; }
 
+// One or two rows whose planes a CTA holds beside its rings: up to 28992 inputs of one, 14464 of two.
+bool planes_fit(const Q4GemvArgs& a) {
+    static_assert(Cfg<0, 1, 32>::FIXED == Cfg<0, 1, 64>::FIXED && Cfg<0, 1, 32>::FIXED == Cfg<0, 1, 128>::FIXED, "one rule for all groups");
+    return a.M <= 2 && Cfg<0, 1, 32>::FIXED + plane_bytes(a) <= SMEM_MAX;
+}
+
 template <int MT, int NT, int G>
 cudaError_t launch(const Q4GemvArgs& a, int sm_count, cudaStream_t s) {
     using C = Cfg<MT, NT, G>;
@@ -440,7 +446,7 @@ cudaError_t launch_rows(const Q4GemvArgs& a, int sm_count, cudaStream_t s) {
 
 template <int G>
 cudaError_t launch_group(const Q4GemvArgs& a, int sm_count, cudaStream_t s) {
-    if (a.M <= 2 && Cfg<0, 1, G>::FIXED + plane_bytes(a) <= SMEM_MAX) {
+    if (planes_fit(a)) {
         // two blocks of outputs share the reads of x's planes where every CTA has several of them (128256 outputs 32.9 us with one,
         // 30.7 with two; 20000 and 40000 the same)
         return blocks_of(a.N, 16) >= 8 * sm_count && Cfg<0, 2, G>::FIXED + plane_bytes(a) <= 112 * 1024 ? launch<0, 2, G>(a, sm_count, s) : launch<0, 1, G>(a, sm_count, s);
@@ -460,7 +466,12 @@ cudaError_t launch_q4_gemv(const Q4GemvArgs& a, int sm_count, cudaStream_t s) {
     // 64 x 60000 14 / 8, 2048 x 8192 9.9 / 8.4); from three on where a warp's slice is long (8 rows: 2048 x 8192 5.7 / 8.2, 8192 x 2048 10.4 / 10.9,
     // 11000 x 5000 33 / 18).
     const bool small = a.K <= 1024 && a.N <= 8192 && a.K * a.N <= 4 << 20;
-    if (a.M > 8 * MAX_MT || (a.M > 8 && !small) || (a.M > 2 && a.K > 8192)) return launch_q4_rows(a, stored_groups(a.K, a.group), sm_count, s);
+    // One or two rows whose planes do not fit there: groups of 64 and 128 (two rows: 14528 x 4096 23.1 / 20.2, 16384 x 2048 21.7 / 17.1,
+    // 28672 x 8192 59 / 53, 28672 x 9600 112 / 70, 28672 x 28672 221 / 197, 14528 x 20000 93 / 102; one: 30000 x 2048 39 / 29, 40000 x 5000
+    // 116 / 50); groups of 32, whose sums it reads out twice as often, stay (two rows: 14528 x 4096 22.4 / 27.8, 28672 x 8192
+    // 62 / 76, 28672 x 28672 236 / 297, 28672 x 1000 39.5 / 38.5, 28672 x 9600 118 / 100; one: 30000 x 2048 40 / 41).
+    const bool wide = a.M > 2 ? a.K > 8192 : !planes_fit(a) && a.group > 32;
+    if (a.M > 8 * MAX_MT || (a.M > 8 && !small) || wide) return launch_q4_rows(a, stored_groups(a.K, a.group), sm_count, s);
     return a.group == 32 ? launch_group<32>(a, sm_count, s) : a.group == 64 ? launch_group<64>(a, sm_count, s) : launch_group<128>(a, sm_count, s);
 }
 
