@@ -31,6 +31,8 @@
 
 #include <algorithm>
 #include <atomic>
+#include <cmath>
+#include <limits>
 #include <new>
 #include <vector>
 
@@ -483,7 +485,9 @@ size_t packed_bytes(int K, int N) { return (size_t)N * ((K + 1) / 2); }
 size_t scale_count(int K, int N, int group) { return (size_t)N * blocks_of(K, group); }
 int grid_of(long long items) { return (int)std::min<long long>((items + 255) / 256, 16384); }
 
-// As the Q8_0 quantiser: per output and group scale = max|w| / 7 (1 for an all-zero group), round to nearest even.
+// As the Q8_0 quantiser: per output and group scale = max|w| / 7 (1 for an all-zero group), round to nearest even.  Groups of
+// tiny values, which that one has no rule for: a scale is fp32's smallest step at least, and where 1 / scale overflows the
+// values are divided (0 times infinity would be no zero).
 void quantize_q4(const float* w, int K, int N, int group, uint8_t* packed, float* scales) {
     const int groups = blocks_of(K, group), bytes = (K + 1) / 2;
     for (int n = 0; n < N; ++n) {
@@ -493,10 +497,11 @@ void quantize_q4(const float* w, int K, int N, int group, uint8_t* packed, float
             const int base = g * group, lim = std::min(base + group, K);
             float max_abs = 0.0f;
             for (int k = base; k < lim; ++k) max_abs = std::max(max_abs, fabsf(w[(size_t)k * N + n]));
-            const float scale = max_abs > 0.0f ? max_abs / 7.0f : 1.0f, inv = 1.0f / scale;
+            const float scale = max_abs > 0.0f ? std::max(max_abs / 7.0f, std::numeric_limits<float>::denorm_min()) : 1.0f, inv = 1.0f / scale;
+            const bool tiny = !std::isfinite(inv);
             scales[(size_t)n * groups + g] = scale;
             for (int k = base; k < lim; ++k) {
-                const float v = std::min(7.0f, std::max(-7.0f, nearbyintf(w[(size_t)k * N + n] * inv)));
+                const float v = std::min(7.0f, std::max(-7.0f, nearbyintf(tiny ? w[(size_t)k * N + n] / scale : w[(size_t)k * N + n] * inv)));
                 const uint8_t u = (uint8_t)((int)v + 8);
                 row[k / 2] = (uint8_t)((k & 1) ? (row[k / 2] & 0x0f) | (u << 4) : (row[k / 2] & 0xf0) | u);
             }
