@@ -458,8 +458,8 @@ int shainet_attn_paged_gather_dev(shainet_attn_ctx* ctx, shainet_attn_paged* pag
  * last group of an output may be short.  Exchange layout: packed [N, ceil(K/2)], K = 2j in the low and 2j + 1 in the
  * high nibble of byte j (the high nibble behind an odd K is ignored and exported as 8), scales [N, ceil(K/group)].
  * q4_create quantises an fp32 matrix [K, N] as the Q8_0 one does: scale = max|w| / 7 (1 for an all-zero group), value =
- * round(w * (1 / scale)), ties to even (w / scale where 1 / scale overflows).  create_raw takes host arrays, create_dev device arrays (read on the context's
- * stream before it returns).  All of them lay the nibbles out anew for the kernel.
+ * round(w * (1 / scale)), ties to even (w / scale where 1 / scale overflows); a weight that is not finite is refused.
+ * create_raw takes host arrays, create_dev device arrays (read on the context's stream before it returns).  All of them lay the nibbles out anew for the kernel.
  * y[rows, N] = x[rows, K] . dequant(W), fp32 sums of exact products; x is not rounded.  x and y do not overlap.  A value
  * of x that is not finite makes its row's outputs not finite and leaves the other rows alone.  Any stream, several at
  * once; nothing is allocated by a product.  The caller synchronises its streams before q4_destroy. */

@@ -487,8 +487,8 @@ int grid_of(long long items) { return (int)std::min<long long>((items + 255) / 2
 
 // As the Q8_0 quantiser: per output and group scale = max|w| / 7 (1 for an all-zero group), round to nearest even.  Groups of
 // tiny values, which that one has no rule for: a scale is fp32's smallest step at least, and where 1 / scale overflows the
-// values are divided (0 times infinity would be no zero).
-void quantize_q4(const float* w, int K, int N, int group, uint8_t* packed, float* scales) {
+// values are divided (0 times infinity would be no zero).  False where a weight is not finite: no nibble stands for it.
+bool quantize_q4(const float* w, int K, int N, int group, uint8_t* packed, float* scales) {
     const int groups = blocks_of(K, group), bytes = (K + 1) / 2;
     for (int n = 0; n < N; ++n) {
         uint8_t* row = packed + (size_t)n * bytes;
@@ -496,7 +496,10 @@ void quantize_q4(const float* w, int K, int N, int group, uint8_t* packed, float
         for (int g = 0; g < groups; ++g) {
             const int base = g * group, lim = std::min(base + group, K);
             float max_abs = 0.0f;
-            for (int k = base; k < lim; ++k) max_abs = std::max(max_abs, fabsf(w[(size_t)k * N + n]));
+            for (int k = base; k < lim; ++k) {
+                if (!std::isfinite(w[(size_t)k * N + n])) return false;
+                max_abs = std::max(max_abs, fabsf(w[(size_t)k * N + n]));
+            }
             const float scale = max_abs > 0.0f ? std::max(max_abs / 7.0f, std::numeric_limits<float>::denorm_min()) : 1.0f, inv = 1.0f / scale;
             const bool tiny = !std::isfinite(inv);
             scales[(size_t)n * groups + g] = scale;
@@ -507,6 +510,7 @@ void quantize_q4(const float* w, int K, int N, int group, uint8_t* packed, float
             }
         }
     }
+    return true;
 }
 
 int check_shape(int K, int N, int group) {
@@ -578,7 +582,7 @@ int shainet_attn_q4_create(shainet_attn_ctx* ctx, shainet_attn_q4** out, const f
     } catch (const std::bad_alloc&) {
         return fail(SHAINET_ATTN_E_NOMEM, "out of host memory");
     }
-    quantize_q4(w, K, N, group, q.data(), sc.data());
+    if (!quantize_q4(w, K, N, group, q.data(), sc.data())) return fail(SHAINET_ATTN_E_INVALID, "a weight is not finite");
     return create_from(ctx, out, q.data(), sc.data(), K, N, group, true);
 }
 

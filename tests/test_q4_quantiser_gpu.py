@@ -1,4 +1,4 @@
-"""Weights that the 4-bit quantiser can only just represent."""
+"""Weights that the 4-bit quantiser can only just represent, and those that it cannot."""
 import numpy as np
 import pytest
 
@@ -34,3 +34,14 @@ def test_quantiser_of_tiny_and_huge_groups(ctx, size):
     assert (got[::5][w[::5] == 0] == 0).all()
     assert np.abs(got - w).max() <= (0.5 + 3 * 7.5 * 2.0 ** -24) * scales.max() + 8 * 2.0 ** -149
     W.close()
+
+
+@pytest.mark.parametrize("bad", [np.nan, np.inf, -np.inf])
+def test_weights_that_are_not_finite_are_refused(ctx, bad):
+    import shainet_b200 as S
+    from shainet_b200 import _lib
+    w = np.ones((70, 5), np.float32)
+    w[69, 4] = bad
+    with pytest.raises(S.ShainetAttnError) as e:
+        S.Q4Weight.from_simple(ctx, w, 64)
+    assert e.value.code == _lib.E_INVALID and "not finite" in str(e.value)
