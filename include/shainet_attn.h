@@ -462,7 +462,8 @@ int shainet_attn_paged_gather_dev(shainet_attn_ctx* ctx, shainet_attn_paged* pag
  * create_raw takes host arrays, create_dev device arrays (read on the context's stream before it returns).  All of them lay the nibbles out anew for the kernel.
  * y[rows, N] = x[rows, K] . dequant(W), fp32 sums of exact products; x is not rounded.  x and y do not overlap.  A value
  * of x that is not finite makes its row's outputs not finite and leaves the other rows alone.  Any stream, several at
- * once; nothing is allocated by a product.  The caller synchronises its streams before q4_destroy. */
+ * once; nothing is allocated by a product.  The caller synchronises its streams before q4_destroy, which
+ * may come after ctx_destroy. */
 typedef struct shainet_attn_q4 shainet_attn_q4;
 int shainet_attn_q4_create(shainet_attn_ctx* ctx, shainet_attn_q4** out, const float* w_host, int K, int N, int group);
 int shainet_attn_q4_create_raw(shainet_attn_ctx* ctx, shainet_attn_q4** out, const uint8_t* packed_host,

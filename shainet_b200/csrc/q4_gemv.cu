@@ -42,6 +42,7 @@ using namespace shainet;
 
 struct shainet_attn_q4 {
     shainet_attn_ctx* ctx = nullptr;
+    int device = 0;
     int K = 0, N = 0, group = 32;
     uint4* q = nullptr;        // [N / 16][K / 64][32 lanes], rounded up
     float* scales = nullptr;   // [N / 16][groups][8][2], rounded up
@@ -530,6 +531,7 @@ int create_from(shainet_attn_ctx* ctx, shainet_attn_q4** out, const uint8_t* pac
     shainet_attn_q4* w = new (std::nothrow) shainet_attn_q4();
     if (!w) return fail(SHAINET_ATTN_E_NOMEM, "out of host memory");
     w->ctx = ctx;
+    w->device = ctx->device;
     w->K = K;
     w->N = N;
     w->group = group;
@@ -596,8 +598,8 @@ int shainet_attn_q4_create_dev(shainet_attn_ctx* ctx, shainet_attn_q4** out, con
 
 int shainet_attn_q4_destroy(shainet_attn_q4* w) {
     if (!w) return SHAINET_ATTN_OK;
-    DeviceGuard g(w->ctx->device);
-    cudaStreamSynchronize(w->ctx->stream);
+    DeviceGuard g(w->device);      // not the context's: it may be gone
+    cudaDeviceSynchronize();
     if (w->q) cudaFree(w->q);
     if (w->scales) cudaFree(w->scales);
     cudaGetLastError();
