@@ -460,8 +460,9 @@ int shainet_attn_paged_gather_dev(shainet_attn_ctx* ctx, shainet_attn_paged* pag
  * q4_create quantises an fp32 matrix [K, N] as the Q8_0 one does: scale = max|w| / 7 (1 for an all-zero group), value =
  * round(w * (1 / scale)), ties to even (w / scale where 1 / scale overflows); a weight that is not finite is refused.
  * create_raw takes host arrays, create_dev device arrays (read on the context's stream before it returns).  All of them lay the nibbles out anew for the kernel.
- * y[rows, N] = x[rows, K] . dequant(W), fp32 sums of exact products; x is not rounded.  x and y do not overlap.  A value
- * of x that is not finite makes its row's outputs not finite and leaves the other rows alone.  Any stream, several at
+ * y[rows, N] = x[rows, K] . dequant(W), fp32 sums of exact products; x is not rounded.  x and y do not overlap.  A group is
+ * summed before its scale is applied: |x| up to 2^117 keeps that sum finite.  Below 2^-110 a value is cut to a multiple of
+ * 2^-133.  A value of x that is not finite makes its row's outputs not finite and leaves the other rows alone.  Any stream, several at
  * once; nothing is allocated by a product.  The caller synchronises its streams before q4_destroy, which
  * may come after ctx_destroy. */
 typedef struct shainet_attn_q4 shainet_attn_q4;

@@ -10,8 +10,10 @@
 //
 // Arithmetic.  The weights are exact as bfloat16: a nibble is dropped into the mantissa of 128 and 136 subtracted (4
 // instructions for 4 values).  Activations are fp32 and enter as three bfloat16 planes each, x = hi + mid + lo exactly (24
-// bits cut into 8 + 8 + 8), so no operand is rounded.  m16n8k16 multiplications with fp32 accumulators; the sums of 32
-// or 64 inputs start from zero and are added in fp32 with their scale, so sums that the matrix units cut off stay short.
+// bits cut into 8 + 8 + 8; below 2^-110 the last of them lie under bfloat16's smallest step, 2^-133), so no operand is rounded.
+// m16n8k16 multiplications with fp32 accumulators; the sums of a whole group with one or two rows, of 32 inputs with more, start
+// from zero and are added in fp32 with their scale, so sums that the matrix units cut off stay short, 128 inputs at most, and
+// finite for |x| up to 2^117 (128 products of up to 8 |x|).
 //   * One or two rows: the planes are the columns of one multiplication (2 rows x 3 planes of 8).
 //   * Up to 24 rows: eight rows a multiplication, three of them for the planes.  More rows, and most products of more than
 //     eight, are taken by q4_rows_tc.cu.

@@ -3,7 +3,7 @@
 //
 // A CTA computes 256 outputs of up to NT rows, as two halves of 128.  The weights are the A operand: a thread owns an
 // output, unpacks 64 of its nibbles at a time into bfloat16 (exact) and puts them into tensor memory.  The rows are the B
-// operand: fp32 values as three bfloat16 planes (exact), made in the CTA, side by side as 3 NT columns of one
+// operand: fp32 values as three bfloat16 planes (exact, as in q4_gemv.cu), made in the CTA, side by side as 3 NT columns of one
 // multiplication.  The sums of 32 (groups of 32), 64 or 128 inputs start from zero in tensor memory; the accumulating warps, a
 // thread an output again, add the three columns of a row and multiply by the group's scale in fp32.
 //
