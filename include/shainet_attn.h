@@ -433,10 +433,11 @@ int shainet_attn_paged_destroy(shainet_attn_paged* paged);
  * behind a plan these are the decode_lens of paged_step_dev, not its lens_out.  Lengths are read on the device, so
  * the call can be captured and replayed as requests grow.  A length that the table cannot hold makes a row of zeros, a
  * table cell outside the pool is not followed (that request's out row is then unspecified); either is reported as
- * SHAINET_ATTN_E_INVALID by the next blocking call on ctx after the stream was synchronised, or, where a kernel also gave up on
- * a wait, by the one behind the call that says so (what the call of one request reports does not touch the others).  Rows of pages behind a request's last position are never used, whatever they
- * hold; projections and rows that a request sees are finite (one that is not makes that request's outputs NaN).  Sums
- * and softmax statistics are fp32; 16-bit rows are multiplied exactly, fp32 rows with operands rounded to 22 bits (2^-23),
+ * SHAINET_ATTN_E_INVALID by the next blocking call on ctx after the stream was synchronised, or, where a kernel also gave up
+ * on a wait, by the one behind the call that says so (what the call of one request reports does not touch the others).
+ * Rows of pages behind a request's last position are never used, whatever they hold.  Projections and rows that a request
+ * sees, and their scores, are finite: where one is not, that request's out row is unspecified (finite or not, so it is no
+ * sign to look for), the other requests' rows are what they are without it.  Sums and softmax statistics are fp32; 16-bit rows are multiplied exactly, fp32 rows with operands rounded to 22 bits (2^-23),
  * as exact as a plain fp32 loop over them.  The batch changes a result only through where a request's positions are
  * split.  No log-sum-exp values are written (set_lse_out) and no peers are served (comm_set_target). */
 int shainet_attn_paged_decode_dev(shainet_attn_ctx* ctx, shainet_attn_paged* paged, const shainet_attn_kv* kv,
