@@ -437,9 +437,11 @@ int shainet_attn_paged_destroy(shainet_attn_paged* paged);
  * on a wait, by the one behind the call that says so (what the call of one request reports does not touch the others).
  * Rows of pages behind a request's last position are never used, whatever they hold.  Projections and rows that a request
  * sees, and their scores, are finite: where one is not, that request's out row is unspecified (finite or not, so it is no
- * sign to look for), the other requests' rows are what they are without it.  Sums and softmax statistics are fp32; 16-bit rows are multiplied exactly, fp32 rows with operands rounded to 22 bits (2^-23),
- * as exact as a plain fp32 loop over them.  The batch changes a result only through where a request's positions are
- * split.  No log-sum-exp values are written (set_lse_out) and no peers are served (comm_set_target). */
+ * sign to look for), the other requests' rows are what they are without it.  Sums and softmax statistics are fp32; 16-bit
+ * rows are multiplied exactly, fp32 rows with operands rounded to 22 bits (2^-22 at most; with more than eight query heads
+ * per kv head a product also lacks what both operands hold below their upper 11 bits, 2^-20 of it at most and 2^-23 on
+ * average), which measures as exact as a plain fp32 loop.  The batch changes a result only through where a request's
+ * positions are split.  No log-sum-exp values are written (set_lse_out) and no peers are served (comm_set_target). */
 int shainet_attn_paged_decode_dev(shainet_attn_ctx* ctx, shainet_attn_paged* paged, const shainet_attn_kv* kv,
                                   void* k_pages, void* v_pages, int num_pages, const float* q_dev, const float* k_new_dev,
                                   const float* v_new_dev, float* out_dev, const int32_t* block_table, int table_width,
@@ -460,12 +462,13 @@ int shainet_attn_paged_gather_dev(shainet_attn_ctx* ctx, shainet_attn_paged* pag
  * high nibble of byte j (the high nibble behind an odd K is ignored and exported as 8), scales [N, ceil(K/group)].
  * q4_create quantises an fp32 matrix [K, N] as the Q8_0 one does: scale = max|w| / 7 (1 for an all-zero group), value =
  * round(w * (1 / scale)), ties to even (w / scale where 1 / scale overflows); a weight that is not finite is refused.
- * create_raw takes host arrays, create_dev device arrays (read on the context's stream before it returns).  All of them lay the nibbles out anew for the kernel.
+ * create_raw takes host arrays, create_dev device arrays (read on the context's stream before it returns).  All of them
+ * lay the nibbles out anew for the kernel.
  * y[rows, N] = x[rows, K] . dequant(W), fp32 sums of exact products; x is not rounded.  x and y do not overlap.  A group is
  * summed before its scale is applied: |x| up to 2^117 keeps that sum finite.  Below 2^-110 a value is cut to a multiple of
- * 2^-133.  A value of x that is not finite makes its row's outputs not finite and leaves the other rows alone.  Any stream, several at
- * once; nothing is allocated by a product.  The caller synchronises its streams before q4_destroy, which
- * may come after ctx_destroy. */
+ * 2^-133.  A value of x that is not finite makes its row's outputs not finite and leaves the other rows alone.  Any stream,
+ * several at once; nothing is allocated by a product.  The caller synchronises its streams before q4_destroy, which may
+ * come after ctx_destroy. */
 typedef struct shainet_attn_q4 shainet_attn_q4;
 int shainet_attn_q4_create(shainet_attn_ctx* ctx, shainet_attn_q4** out, const float* w_host, int K, int N, int group);
 int shainet_attn_q4_create_raw(shainet_attn_ctx* ctx, shainet_attn_q4** out, const uint8_t* packed_host,

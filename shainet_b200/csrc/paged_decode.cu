@@ -26,8 +26,10 @@
 //    exactly (24 bits cut into 8 + 8 + 8): no operand is rounded.  The planes lie side by side in the 16 rows of one
 //    multiplication: four heads' three planes in one, eight heads' in two, sixteen heads' in three.
 //  * fp32 rows (m16n8k8, TF32): every operand enters as two planes of 11 bits, hi + lo, so an operand keeps 22 of its 24
-//    bits, rounded (2^-23 relative); the sum of head_dim products of it is about as exact as the fp32 sum of a plain loop,
-//    whose own roundings are of that size.  Eight heads' planes take one multiplication with each plane of the rows.
+//    bits, rounded: of x in [1, 2) the upper plane leaves less than 2^-10, whose 11 bits end at 2^-21, so 2^-22 is lost at
+//    most.  The sum of head_dim products of it is about as exact as the fp32 sum of a plain loop, whose own roundings are of
+//    that size.  Eight heads' planes take one multiplication with each plane of the rows.  Sixteen heads take three, and
+//    leave out the product of the two lower planes: 2^-20 of a product at most, 2^-23 on average.
 // P.V of each tile starts from zero and is added to the running sum in fp32 with the rescaling, so that sums that the
 // matrix units cut off stay one tile long.
 //
