@@ -382,8 +382,8 @@ int shainet_attn_decode_noalloc(const float* q_dev, const float* k_cache_dev, co
  * the element format of SHAINET_ATTN_KV_*; and, shared by all blocks, block_table [requests, table_width] int32 whose
  * row r lists the pages of request r in order, and lens [requests] int32.  Position p of request r lies in row
  * p % page_rows of page block_table[r][p / page_rows]; the slot of a position is page * page_rows + row.  A page belongs
- * to one request where rows are written into it; pages that are only read may be shared.  num_pages * page_rows is at
- * most 2^31 - 1, page_rows 1 .. 4096.
+ * to one request where rows are written into it; decode and gather may be given tables that share pages which are only
+ * read, plan_dev may not.  num_pages * page_rows is at most 2^31 - 1, page_rows 1 .. 4096.
  *
  * plan_dev: one step of the page tables, on the device and in one launch.  Request r holds lens[r] positions; delta[r]
  * positions are added (> 0) or the newest ones dropped (< 0; -lens[r] ends the request).  The free pages are a stack,
@@ -391,13 +391,16 @@ int shainet_attn_decode_noalloc(const float* q_dev, const float* k_cache_dev, co
  * by their place in its table; then requests that grow pop theirs in the order of the requests, by place in the table.
  * Written: the new table cells, the stack, lens_out = lens + delta, free_count_out, first [requests + 1] (the exclusive
  * sums of max(delta, 0): where a request's new tokens start), slots [max_tokens] (the slot of every new token, -1 behind
- * the last one and for a page outside the pool) and status [2].  Table cells and stack entries that are not in use keep what they held.  lens_out may be
- * lens and free_count_out may be free_count (a captured step advances its own state); no other two arrays may overlap.
+ * the last one and for a page outside the pool) and status [2].  Table cells and stack entries that are not in use keep
+ * what they held.  lens_out may be lens and free_count_out may be free_count (a captured step advances its own state); no
+ * other two arrays may overlap.
  * Nothing is changed (lens_out = lens, free_count_out = free_count, first 0, slots -1) and status[0] is not 0 where
  * the step cannot be taken: SHORT, status[1] pages are missing; LENGTH, request status[1] has a length below 0 or above
  * table_width * page_rows before or after the step; TOKENS, the status[1] new tokens are more than max_tokens; STACK,
  * free_count[0] = status[1] is outside [0, num_pages], or the stack would outgrow free_pages [num_pages].
- * requests is at most SHAINET_ATTN_PAGED_MAX_REQUESTS.  free_pages holds each free page once. */
+ * requests is at most SHAINET_ATTN_PAGED_MAX_REQUESTS.  free_pages holds each free page once, and no page is in two
+ * requests' tables or in a table and on the stack: pages have no counts, so each request that ends or shrinks pushes its own,
+ * and one that two requests share would be handed out twice.  Who shares pages keeps the tables and the free list. */
 #define SHAINET_ATTN_PAGED_MAX_REQUESTS 8192
 #define SHAINET_ATTN_PLAN_OK 0
 #define SHAINET_ATTN_PLAN_SHORT 1
