@@ -453,7 +453,9 @@ int shainet_attn_paged_decode_dev(shainet_attn_ctx* ctx, shainet_attn_paged* pag
  * (shainet_attn_forward_dev).  scatter: rows row0 .. row0 + rows - 1 of kv go to slots[0 .. rows) (distinct; a negative
  * slot is skipped).  gather: positions 0 .. rows - 1 of the request whose table row is table_row become the rows of kv,
  * whose length becomes rows; kv grows if it has to, which a stream that is being captured does not allow.  A slot or
- * page outside the pool is skipped and reported as above. */
+ * page outside the pool is skipped and reported as above.  table_row holds a page for every page_rows positions of rows.
+ * What a stream captures holds the cache's memory as it was: a cache whose rows a graph copies is not grown (reserve it
+ * first, or use kv_create_reserved) or destroyed while the graph may be replayed, and its length is the host's business. */
 int shainet_attn_paged_scatter_dev(shainet_attn_ctx* ctx, shainet_attn_paged* paged, const shainet_attn_kv* kv, void* k_pages,
                                    void* v_pages, int num_pages, const int32_t* slots, int row0, int rows, void* stream);
 int shainet_attn_paged_gather_dev(shainet_attn_ctx* ctx, shainet_attn_paged* paged, shainet_attn_kv* kv, const void* k_pages,

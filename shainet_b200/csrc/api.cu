@@ -381,7 +381,7 @@ bool single_token_rows(const shainet_attn_ctx* ctx, const HeadShape& hs, unsigne
 struct Ahead {
     bool rewound = false, refilled = false;
 };
-Ahead ahead_of(const shainet_attn_kv* kv) { return Ahead{kv->rewound, kv->refilled}; }
+Ahead ahead_of(const shainet_attn_kv* kv) { return Ahead{kv->rewound, kv->refilled || kv->refilled_by_graph}; }
 // Every launch waits for what was enqueued before it in its stream, and lets its successor in only then.
 void launched(shainet_attn_kv* kv) { kv->rewound = kv->refilled = false; }
 
@@ -1294,8 +1294,9 @@ int shainet_attn_forward_batched_dev(shainet_attn_ctx* ctx, shainet_attn_kv* con
     int max_visible = 0;
     Ahead ahead;
     for (int b = 0; b < batch; ++b) {
-        ahead.rewound |= kvs[b]->rewound;
-        ahead.refilled |= kvs[b]->refilled;
+        const Ahead one = ahead_of(kvs[b]);
+        ahead.rewound |= one.rewound;
+        ahead.refilled |= one.refilled;
         hd[b] = SeqDesc{kvs[b]->k, kvs[b]->v, kvs[b]->len, kvs[b]->cap};
         total_visible += kvs[b]->len + 1;
         max_visible = std::max(max_visible, kvs[b]->len + 1);

@@ -89,6 +89,7 @@ struct shainet_attn_kv {
                                 // launch ahead still reads, so it must not run ahead of it (F_INPUTS_READY is ignored once)
     bool refilled = false;      // a copy out of pages has written rows since the last launch on this cache and may still run: the
                                 // next launch reads no row, and takes no input for granted, ahead of its wait for it
+    bool refilled_by_graph = false;   // such a copy was captured: its graph may be replayed ahead of any launch on this cache
     float* inv_freq = nullptr;  // device, head_dim/2
     float* q_norm = nullptr;    // device, nullable
     float* k_norm = nullptr;

@@ -254,13 +254,14 @@ int shainet_attn_paged_gather_dev(shainet_attn_ctx* ctx, shainet_attn_paged* pag
                                               kv->pages_per_head * kv->page_bytes
                                         : rows > kv->cap || !kv->k;
         cudaStreamCaptureStatus capture = cudaStreamCaptureStatusNone;
-        if (grows) CU(cudaStreamIsCapturing(s, &capture));
-        if (capture != cudaStreamCaptureStatusNone)
+        CU(cudaStreamIsCapturing(s, &capture));
+        if (grows && capture != cudaStreamCaptureStatusNone)
             return fail(SHAINET_ATTN_E_STATE, "the cache cannot grow to %d rows on a stream that is being captured", rows);
         rc = kv_ensure_rows(kv, rows, s);
         if (!rc)
             rc = copy_rows(ctx, paged, kv, const_cast<void*>(k_pages), const_cast<void*>(v_pages), num_pages, table_row, 0, rows, false, s);
         if (rc) return rc;
+        if (capture != cudaStreamCaptureStatusNone) kv->refilled_by_graph = true;
     }
     kv->refilled = true;
     kv->len = rows;

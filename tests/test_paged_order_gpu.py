@@ -143,6 +143,34 @@ def test_a_batch_with_one_refilled_cache(ctx, kv):
     t.close()
 
 
+@pytest.mark.parametrize("kv", ["f32", "bf16"])
+def test_tokens_behind_replays_of_a_captured_copy(ctx, kv):
+    """A graph fills the cache, an eager token follows, over and over: the graph's copies are not seen by the host."""
+    import torch
+    import shainet_b200 as S
+    t = Turns(ctx, SHAPES["Q8B"], 2500, 16, kv)
+    want, graphs = [], [torch.cuda.CUDAGraph() for _ in range(2)]
+    for which in (0, 1):
+        t.gather(which)
+        t.wait()
+        want.append(t.new())
+        t.token(want[-1])
+        t.wait()
+        with torch.cuda.graph(graphs[which], stream=t.stream):
+            t.gather(which)
+    outs = [t.new() for _ in range(40)]
+    with torch.cuda.stream(t.stream):
+        for i, out in enumerate(outs):
+            t.attn.cache.truncate(2500)
+            graphs[i & 1].replay()
+            t.token(out, S.F_INPUTS_READY if i & 2 else 0)
+    t.wait()
+    for i, out in enumerate(outs):
+        assert torch.equal(out, want[i & 1]), i
+    del graphs
+    t.close()
+
+
 def test_an_emptied_cache_starts_again(ctx):
     t = Turns(ctx, SHAPES["L1B"], 64, 16, "f32")
     out, ref = t.new(), t.new()
