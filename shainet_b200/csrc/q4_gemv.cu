@@ -9,7 +9,8 @@
 // [group][output g and g + 8].  Outputs are padded to 16 with scale 0, inputs to 64 with value 0.
 //
 // Arithmetic.  The weights are exact as bfloat16: a nibble is dropped into the mantissa of 128 and 136 subtracted (4
-// instructions for 4 values).  Activations are fp32 and enter as three bfloat16 planes each, x = hi + mid + lo exactly (24
+// instructions for 4 values; integers as the low mantissa bits of a power of two that is subtracted again are a published
+// conversion: Kim, Henry, Fahim and Awadalla 2022 for half precision).  Activations are fp32 and enter as three bfloat16 planes each, x = hi + mid + lo exactly (24
 // bits cut into 8 + 8 + 8; below 2^-110 the last of them lie under bfloat16's smallest step, 2^-133), so no operand is rounded.
 // m16n8k16 multiplications with fp32 accumulators; the sums of a whole group with one or two rows, of 32 inputs with more, start
 // from zero and are added in fp32 with their scale, so sums that the matrix units cut off stay short, 128 inputs at most, and
@@ -19,12 +20,13 @@
 //     eight, are taken by q4_rows_tc.cu.
 //
 // Work.  A CTA takes NT blocks of outputs at a time and splits their inputs over its eight warps, each with a ring of its own
-// in shared memory that asynchronous copies fill RING - 1 places ahead; the warps' sums meet in shared memory.  The first
+// in shared memory that asynchronous copies fill RING - 1 places ahead (with one or two rows one place, four blocks of inputs,
+// requested when the one before it has arrived); the warps' sums meet in shared memory.  The first
 // weights are requested before the wait for the kernel ahead in the stream: they never depend on it.
 //
-// Bounds.  One row: 0.5 byte and 4 / group bytes a weight from HBM; the integer pipe is as busy (11 instructions for 8 nibbles):
-// 2048 -> 128256 in groups of 64 takes 30.6 us, 4.8 TB/s or 75 % of a copy's rate, with 53 % of the cycles of that pipe and 58 %
-// of the issue slots taken.  2048 -> 512 takes 2.2 us, a launch.  Several rows: the latency of eight warps an SM, whose rows come from L2 two steps
+// Bounds.  One row: 0.5 byte and 4 / group bytes a weight from HBM, 11 instructions for 8 nibbles.  2048 -> 128256 in groups of 64
+// takes 30.6 to 31.3 us, 4.8 TB/s or 75 % of a copy's rate, with 53 % of the cycles of the integer pipe and 58 % of the issue slots
+// taken: nothing is saturated, a warp waits for its one place in flight and then computes while the next one is under way.  2048 -> 512 takes 2.2 us, a launch.  Several rows: the latency of eight warps an SM, whose rows come from L2 two steps
 // ahead (8 x 2048 -> 8192 5.8 us; one step ahead 6.4 % to 14 % longer from 17 rows on).  Fetching them by asynchronous copies into shared
 // memory was slower, and two scaled half-precision planes instead of three were not faster.
 #include <cuda_runtime.h>

@@ -17,7 +17,7 @@
 // two warpgroups take the blocks of the rows in turn (124 -> 118 us at 64 x 2048 x 128256) and each half has a warp of its own
 // that issues the multiplications, with slots and parities that are constants (one warp for both: 1450 cycles a step).  Rows
 // through registers instead of the ring took 9 % longer, a read-out two places deep as long.
-// Measured: 33 x 2048 -> 8200 10.6 us, 64 x 4096 -> 4096 16.5 us, 64 x 2048 -> 128256 118 us (mma.sync, which takes 8.5 cycles of a
+// Measured: 33 x 2048 -> 8200 10.6 us, 64 x 4096 -> 4096 16.5 us, 64 x 2048 -> 128256 118 to 126 us by the card (mma.sync, which takes 8.5 cycles of a
 // quarter SM for 16 outputs and eight columns: 17.6, 27.4 and 426).  A launch with little to do takes 4.4 us.
 #include <cuda_runtime.h>
 
