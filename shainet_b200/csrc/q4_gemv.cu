@@ -530,6 +530,7 @@ int create_from(shainet_attn_ctx* ctx, shainet_attn_q4** out, const uint8_t* pac
     *out = nullptr;
     int rc = check_shape(K, N, group);
     if (rc) return rc;
+    if (!host && (reinterpret_cast<uintptr_t>(scales) & 3u) != 0) return fail(SHAINET_ATTN_E_INVALID, "device scales must be 4-byte aligned");
     if (!ctx) return fail(SHAINET_ATTN_E_INVALID, "null context");
     DeviceGuard g(ctx->device);
     shainet_attn_q4* w = new (std::nothrow) shainet_attn_q4();
