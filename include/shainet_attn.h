@@ -438,6 +438,8 @@ int shainet_attn_paged_destroy(shainet_attn_paged* paged);
  * table cell outside the pool is not followed (that request's out row is then unspecified); either is reported as
  * SHAINET_ATTN_E_INVALID by the next blocking call on ctx after the stream was synchronised, or, where a kernel also gave up
  * on a wait, by the one behind the call that says so (what the call of one request reports does not touch the others).
+ * Reported so too, with all out rows zeros and no page written: a batch whose requests together read more than about 2^30
+ * tiles of 8 KB (8 TB of rows; tables that share pages could name that many).
  * Rows of pages behind a request's last position are never used, whatever they hold.  Projections and rows that a request
  * sees, and their scores, are finite: where one is not, that request's out row is unspecified (finite or not, so it is no
  * sign to look for), the other requests' rows are what they are without it.  Sums and softmax statistics are fp32; 16-bit

@@ -1,6 +1,6 @@
 """Attention over pages where one request's visible rows or projections are not finite: the others' outputs and pages are,
 bit for bit, what they are without it.  The requests share the line of tiles, so the CTAs that work on the bad one also work on
-its neighbours."""
+its neighbours.  And batches that name more rows than there can be."""
 import numpy as np
 import pytest
 
@@ -55,3 +55,41 @@ def test_one_bad_request_leaves_the_others_alone(ctx, layout, lens, kv):
             for g, c in zip(got[1:], clean[1:]):
                 assert np.array_equal(g[keep], c[keep], equal_nan=True), (value, what)
     b.close()
+
+
+@pytest.mark.parametrize("kv", ["f32", "bf16"])
+def test_more_rows_than_there_can_be(ctx, kv):
+    """Tables that name the same pages over and over: 2^31 - 1 positions of one request, and 999 of sixteen million each,
+    are more than the line of tiles holds.  All rows are zeros, no page is written, the call says so and the next one works."""
+    import torch
+    import shainet_b200 as S
+    from shainet_b200 import _lib
+    H, KV, hd, P = 16, 8, 128, 4096
+    attn, paged = S.LlamaAttention(ctx, H, KV, hd, kv_format=kv), S.PagedAttention(ctx, H, KV, hd, P, kv)
+    dt = torch.float32 if kv == "f32" else torch.bfloat16
+    kp, vp = (torch.randn(2, KV, P, hd, device="cuda").to(dt) for _ in range(2))
+    before = kp.clone(), vp.clone()
+    for R, W, lens in ((2, 1 << 19, [2**31 - 1, 5]), (1000, 4096, [16000000] * 999 + [7])):
+        table = torch.zeros(R, W, dtype=torch.int32, device="cuda")
+        q, k, v = (torch.randn(R, n * hd, device="cuda") for n in (H, KV, KV))
+        out = torch.full((R, H * hd), float("nan"), device="cuda")
+        tl = torch.tensor(lens, dtype=torch.int32, device="cuda")
+        call = lambda: paged.decode_dev(attn, kp.data_ptr(), vp.data_ptr(), 2, q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(),
+                                        table.data_ptr(), W, tl.data_ptr(), R, 0.1)
+        torch.cuda.synchronize()
+        call()
+        with pytest.raises(S.ShainetAttnError) as e:
+            ctx.sync()
+        assert e.value.code == _lib.E_INVALID
+        assert not out.any() and torch.equal(kp, before[0]) and torch.equal(vp, before[1])
+        tl.zero_()
+        tl[1] = 3
+        out.fill_(float("nan"))
+        torch.cuda.synchronize()
+        call()
+        ctx.sync()
+        assert out[1].isfinite().all() and out[1].any() and not out[0].any()
+        for x, y in zip((kp, vp), before):
+            x.copy_(y)
+    paged.close()
+    attn.close()
