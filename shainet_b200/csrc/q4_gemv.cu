@@ -10,11 +10,11 @@
 //
 // Arithmetic.  The weights are exact as bfloat16: a nibble is dropped into the mantissa of 128 and 136 subtracted (4
 // instructions for 4 values; integers as the low mantissa bits of a power of two that is subtracted again are a published
-// conversion: Kim, Henry, Fahim and Awadalla 2022 for half precision).  Activations are fp32 and enter as three bfloat16 planes each, x = hi + mid + lo exactly (24
-// bits cut into 8 + 8 + 8; below 2^-110 the last of them lie under bfloat16's smallest step, 2^-133), so no operand is rounded.
-// m16n8k16 multiplications with fp32 accumulators; the sums of a whole group with one or two rows, of 32 inputs with more, start
-// from zero and are added in fp32 with their scale, so sums that the matrix units cut off stay short, 128 inputs at most, and
-// finite for |x| up to 2^117 (128 products of up to 8 |x|).
+// conversion: Kim, Henry, Fahim and Awadalla 2022, for half precision).  Activations are fp32 and enter as three bfloat16
+// planes each, x = hi + mid + lo exactly (24 bits cut into 8 + 8 + 8; below 2^-110 the last of them lie under bfloat16's
+// smallest step, 2^-133), so no operand is rounded.  m16n8k16 multiplications with fp32 accumulators; the sums of a whole
+// group with one or two rows, of 32 inputs with more, start from zero and are added in fp32 with their scale, so sums that
+// the matrix units cut off stay short, 128 inputs at most, and finite for |x| up to 2^117 (128 products of up to 8 |x|).
 //   * One or two rows: the planes are the columns of one multiplication (2 rows x 3 planes of 8).
 //   * Up to 24 rows: eight rows a multiplication, three of them for the planes.  More rows, and most products of more than
 //     eight, are taken by q4_rows_tc.cu.
@@ -24,11 +24,12 @@
 // requested when the one before it has arrived); the warps' sums meet in shared memory.  The first
 // weights are requested before the wait for the kernel ahead in the stream: they never depend on it.
 //
-// Bounds.  One row: 0.5 byte and 4 / group bytes a weight from HBM, 11 instructions for 8 nibbles.  2048 -> 128256 in groups of 64
-// takes 30.6 to 31.3 us, 4.8 TB/s or 75 % of a copy's rate, with 53 % of the cycles of the integer pipe and 58 % of the issue slots
-// taken: nothing is saturated, a warp waits for its one place in flight and then computes while the next one is under way.  2048 -> 512 takes 2.2 us, a launch.  Several rows: the latency of eight warps an SM, whose rows come from L2 two steps
-// ahead (8 x 2048 -> 8192 5.8 us; one step ahead 6.4 % to 14 % longer from 17 rows on).  Fetching them by asynchronous copies into shared
-// memory was slower, and two scaled half-precision planes instead of three were not faster.
+// Bounds.  One row: 0.5 byte and 4 / group bytes a weight from HBM, 11 instructions for 8 nibbles.  2048 -> 128256 in groups
+// of 64 takes 30.6 to 31.3 us, 4.8 TB/s or 75 % of a copy's rate, with 53 % of the cycles of the integer pipe and 58 % of the
+// issue slots taken: nothing is saturated, a warp waits for its one place in flight and then computes while the next one is
+// under way.  2048 -> 512 takes 2.2 us, a launch.  Several rows: the latency of eight warps an SM, whose rows come from L2
+// two steps ahead (8 x 2048 -> 8192 5.8 us; one step ahead 6.4 % to 14 % longer from 17 rows on).  Fetching them by
+// asynchronous copies into shared memory was slower, and two scaled half-precision planes instead of three were not faster.
 #include <cuda_runtime.h>
 #include <math.h>
 #include <stdint.h>
